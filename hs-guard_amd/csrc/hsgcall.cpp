@@ -87,6 +87,10 @@ PyMethodDef methods[] = {HSG_ENTRY(hsg_gdn_slot_step),
                          HSG_ENTRY(hsg_gemm_bf16_skinny),
                          HSG_ENTRY(hsg_gemm_bf16_skinny_silu),
                          HSG_ENTRY(hsg_gemm_bf16_skinny_addnorm),
+                         HSG_ENTRY(hsg_tree_maps),
+                         HSG_ENTRY(hsg_tree_conv_silu),
+                         HSG_ENTRY(hsg_gdn_tree_step),
+                         HSG_ENTRY(hsg_tree_attention),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hsgcall", "Entry points of libhsg.so", -1, methods, nullptr, nullptr, nullptr,

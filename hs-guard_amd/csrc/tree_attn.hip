@@ -1,0 +1,616 @@
+// Window attention of a drafted tree's nodes over the slot's ring and each node's own ancestors, gated, for gfx950 on MFMA.
+//
+// Node i of a row stands at start + depth_i. It sees the ring's keys at 0 <= p < start, p > start + depth_i - W, and of the
+// tree's keys those of its ancestors and its own that lie within W of it. Nothing of the ring moves but, in a second launch
+// after all reads, the columns of the committed chain.
+//
+// Query rows r = node * G + (query head of the kv head) form tiles of 16. A workgroup of 4 waves takes one (row, kv head) and
+// 16 T QW query rows, as QW x KW waves (QW KW = 4): the KW waves of a query group split the KEYS, blocks of 32 in turn, so a
+// wave's keys and values go straight from memory to its operand registers, each read once for its T tiles, with no LDS, no
+// barrier and no wave waiting for another in the loop. Per block, on v_mfma_f32_16x16x32_bf16:
+//   S^T[key, query] = K . Q^T      a lane's column is one query: maxima, sums and rescales are per-lane scalars
+//   O^T[d, query] += V^T . P^T     B = P straight from the S^T accumulators (the product's key order is the lane's own);
+//                                  A = V^T: a lane reads 8 dims of its 8 keys and swaps 16-bit halves in registers, product
+//                                  i of 8 taking dim 8 c + i of each lane c
+// The running maximum is moved only when a block's exceeds it by 2^8, so the accumulators are seldom rescaled; sums are fp32
+// and P is rounded to bf16 for its product (2^-9 of each weight, below the output's own rounding). At the end the waves'
+// partial sums meet in LDS, weighted by their maxima. Where few rows leave the chip short of workgroups, NS workgroups split
+// a row's key blocks further and a second launch joins their partial sums.
+//
+// A masked pair has P = 0, which would carry a NaN or an infinity of a value to queries that do not see it: values that no
+// query of the workgroup sees are zeroed as they are loaded, and where a result is not finite its lane computes it again from
+// the keys that its query sees alone (walk_keys).
+#include <math.h>
+
+#include "hsg_common.h"
+
+namespace hsg {
+namespace {
+
+constexpr int D = 256;
+constexpr int NW = 4;
+constexpr int KB = 32;                 // keys of a block
+constexpr int W_MAX = 512;
+constexpr int MOST = HSG_TREE_MAX_NODES;
+constexpr int BLOCKS = W_MAX / KB + MOST / KB;
+constexpr int KP_NONE = -(1 << 30);    // an empty ring column
+constexpr int KP_FAR = 1 << 29;        // clamp of a position relative to the row's start
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float SLACK = 8.f;           // log2 of how far a score may exceed the running maximum before it is moved
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+
+struct TreeAttnParams {
+  const uint16_t* q; int64_t q_sl, q_sh, q_sg;
+  uint16_t* ring_k; uint16_t* ring_v; int64_t ring_rows; int W;
+  const uint16_t* new_k; int64_t nk_sl, nk_sh;
+  const uint16_t* new_v; int64_t nv_sl, nv_sh;
+  const uint16_t* gate; int64_t g_sl, g_sh, g_sg, g_off;
+  const int64_t* ring_pos; const int64_t* slots; const int64_t* starts; const int64_t* lens; const int64_t* offsets;
+  const int64_t* commits; const int64_t* masks;
+  int max_nodes, hkv, G;
+  float scale;
+  int pairs;        // rows x kv heads
+  int qblocks;      // workgroups of query rows a pair
+  int splits;       // workgroups of key blocks
+  float* part_o;    // [pair][split][query row][D]: partial sums
+  float* part_ml;   // [pair][split][query row][2]: their maxima and weights' sums
+  uint16_t* out; int64_t o_sl, o_sh, o_sg;
+};
+
+// A (row, kv head): element pointers of its first node
+struct TreeKeys {
+  const uint16_t* q; const uint16_t* k; const uint16_t* v; const uint16_t* gate; uint16_t* out;
+  const uint16_t* ring_k; const uint16_t* ring_v;   // column 0
+  const int64_t* ring_pos; const int64_t* masks;
+  int64_t start;
+  int len;
+};
+
+__device__ __forceinline__ bool tree_keys(const TreeAttnParams& p, int n, int h, TreeKeys& ro) {
+  const int64_t slot = p.slots[n], len = p.lens[n], off = p.offsets[n];
+  ro.start = p.starts[n];
+  if ((slot < 0) | (slot >= p.ring_rows) | (len <= 0) | (len > p.max_nodes)) return false;
+  ro.len = (int)len;
+  ro.q = p.q + off * p.q_sl + h * p.q_sh;
+  ro.k = p.new_k + off * p.nk_sl + h * p.nk_sh;
+  ro.v = p.new_v + off * p.nv_sl + h * p.nv_sh;
+  ro.gate = p.gate ? p.gate + off * p.g_sl + h * p.g_sh + p.g_off : nullptr;
+  ro.out = p.out + off * p.o_sl + h * p.o_sh;
+  const int64_t ring = ((slot * p.hkv + h) * (int64_t)(p.W + 1)) * D;
+  ro.ring_k = p.ring_k + ring;
+  ro.ring_v = p.ring_v + ring;
+  ro.ring_pos = p.ring_pos + slot * (int64_t)(p.W + 1);
+  ro.masks = p.masks + off;
+  return true;
+}
+
+__device__ __forceinline__ bf16x8 as_bf16x8(u32x4 w) { return __builtin_bit_cast(bf16x8, w); }
+__device__ __forceinline__ u32x4 load16(const uint16_t* p) { return *reinterpret_cast<const u32x4*>(p); }
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// node i's ancestors and itself
+__device__ __forceinline__ uint64_t mask_of(const int64_t* masks, int i) {
+  const uint64_t self = 1ull << i;
+  return ((uint64_t)masks[i] & (self - 1)) | self;
+}
+
+// node i's depth
+__device__ __forceinline__ int depth_of(const int64_t* masks, int i) { return (int)__popcll(mask_of(masks, i)) - 1; }
+
+// position of a ring column's key before the row's start, or KP_NONE
+__device__ __forceinline__ int key_place(int64_t kpos, int64_t start) {
+  const int64_t d = kpos - start;
+  return kpos < 0 || d >= 0 ? KP_NONE : (int)(d < -KP_FAR ? -KP_FAR : d);
+}
+
+// ND values (dims d0 ..) of query `row` by definition, over the keys it sees alone
+template <int ND>
+__device__ __forceinline__ void walk_keys(const TreeAttnParams& p, const TreeKeys& ro, int row, int d0, float (&y)[ND]) {
+  const int l = row / p.G;
+  const uint16_t* q = ro.q + l * p.q_sl + (row - l * p.G) * p.q_sg;
+  const uint64_t mask = mask_of(ro.masks, l);
+  const int depth = depth_of(ro.masks, l);
+  const auto key = [&](int j, bool ring) -> const uint16_t* { return ring ? ro.ring_k + j * D : ro.k + j * p.nk_sl; };
+  const auto sees = [&](int j, bool ring) {
+    if (ring) return key_place(ro.ring_pos[j], ro.start) > depth - p.W;
+    return (mask >> j & 1) && depth_of(ro.masks, j) > depth - p.W;
+  };
+  const auto score = [&](const uint16_t* k) {
+    float s = 0.f;
+    for (int d = 0; d < D; d += 8) {
+      float a[8], b[8];
+      load8_bf16(q + d, a);
+      load8_bf16(k + d, b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = __builtin_fmaf(a[e], b[e], s);
+    }
+    return s * p.scale;
+  };
+  float m = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < ND; ++e) y[e] = 0.f;
+  for (int pass = 0; pass < 2; ++pass)
+    for (int j = 0; j < p.W + ro.len; ++j) {
+      const bool ring = j < p.W;
+      const int at = ring ? j : j - p.W;
+      if (!sees(at, ring)) continue;
+      const float s = score(key(at, ring));
+      if (pass == 0) {
+        m = fmaxf(m, s);
+        continue;
+      }
+      const float w = expf(s - m);
+      sum += w;
+      const uint16_t* v = (ring ? ro.ring_v + at * D : ro.v + at * p.nv_sl) + d0;
+      for (int e = 0; e < ND; ++e) y[e] += w * bf2f(v[e]);
+    }
+#pragma unroll
+  for (int e = 0; e < ND; ++e) y[e] /= sum;
+}
+
+template <int ND>
+__device__ __forceinline__ bool all_finite(const float (&y)[ND]) {
+  float odd = 0.f;
+#pragma unroll
+  for (int e = 0; e < ND; ++e) odd += y[e] * 0.f;
+  return odd == 0.f;
+}
+
+// ND normalised values of query `row`, gated and stored (dims d0 ..); not finite: computed again first
+template <int ND>
+__device__ __forceinline__ void finish(const TreeAttnParams& p, const TreeKeys& ro, int row, int d0, float (&y)[ND]) {
+  if (!all_finite(y)) walk_keys(p, ro, row, d0, y);
+  const int l = row / p.G, g = row - l * p.G;
+  uint16_t* dst = ro.out + l * p.o_sl + g * p.o_sg + d0;
+  if (ro.gate) {
+    const uint16_t* src = ro.gate + l * p.g_sl + g * p.g_sg + d0;
+#pragma unroll
+    for (int e = 0; e < ND; e += 8) {
+      float gt[8];
+      load8_bf16(src + e, gt);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[e + i] *= sigmoidf_(gt[i]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < ND; e += 8) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(y[e + 2 * i], y[e + 2 * i + 1]);
+    *reinterpret_cast<u32x4*>(dst + e) = w;
+  }
+}
+
+template <int T, int KW>
+__global__ __launch_bounds__(64 * NW) void tree_attn_kernel(const TreeAttnParams p) {
+  constexpr int QW = NW / KW;
+  constexpr int ROWS = 16 * T * QW;     // query rows of the workgroup
+  constexpr bool Q_LDS = T > 2;         // the queries' operands stay in LDS, in the order of the lanes, not in registers
+  __shared__ union __align__(16) Lds {
+    u32x4 q[QW * T][D / 32][64];
+    f32x4 o[NW][16][64];                // a tile's partial sums of every wave
+    __device__ Lds() {}
+  } lds;
+  __shared__ __align__(16) int kp[W_MAX + MOST];   // places of the ring's keys before the start; then the nodes' depths
+  __shared__ uint32_t flags[BLOCKS];               // bit 0: some query may see a key of the block; 1: all see all
+  __shared__ float ml[NW][T][16][2];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wk = wave % KW, wq = wave / KW;
+  const int g4 = lane >> 4, c = lane & 15;
+  // Workgroups are dealt round-robin over the 8 XCDs: the ones of a pair follow one another on one XCD, whose L2 then serves
+  // its keys to all but the first.
+  const int per = p.qblocks * p.splits;
+  const int seq = blockIdx.x >> 3;
+  const int pair = seq / per * 8 + (blockIdx.x & 7);
+  if (pair >= p.pairs) return;
+  const int part = seq % per;
+  const int qb = part / p.splits, split = part - qb * p.splits;
+  const int n = pair / p.hkv, h = pair - n * p.hkv;
+  TreeKeys ro;
+  if (!tree_keys(p, n, h, ro)) return;
+  const int W = p.W, G = p.G, len = ro.len;
+  const int M = G * len;
+  const int r_wg = qb * ROWS;
+  if (r_wg >= M) return;
+  const int r_lo = r_wg + 16 * T * wq;
+  const int tiles = min(T, max(0, (M - r_lo + 15) >> 4));   // of this wave
+  const int l_hi = (min(r_wg + ROWS, M) - 1) / G;           // last node of the workgroup
+  const int RB = W / KB;
+  const int n_blocks = RB + l_hi / KB + 1;
+
+  // ---- queries, and places of the keys ----
+  bf16x8 qr[Q_LDS ? 1 : T][D / 32];
+  uint64_t mask[T];
+  int depth[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int row = min(r_lo + 16 * t + c, M - 1);           // past the valid rows: the last one again, not stored
+    const int l = row / G;
+    const uint16_t* src = ro.q + l * p.q_sl + (row - l * G) * p.q_sg + 8 * g4;
+    mask[t] = mask_of(ro.masks, l);
+    depth[t] = depth_of(ro.masks, l);
+    if constexpr (!Q_LDS) {
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ++ks) qr[t][ks] = as_bf16x8(load16(src + 32 * ks));
+    } else {
+      // the KW waves of the query group share the work
+#pragma unroll
+      for (int ks = 0; ks < D / 32 / KW; ++ks)
+        lds.q[wq * T + t][wk * (D / 32 / KW) + ks][lane] = load16(src + 32 * (wk * (D / 32 / KW) + ks));
+    }
+  }
+  for (int col = threadIdx.x; col < W_MAX; col += 64 * NW) {
+    const int place = col < W ? key_place(ro.ring_pos[min(col, W - 1)], ro.start) : KP_NONE;
+    kp[col] = place;
+    const uint64_t some = __ballot(place > -W), all = __ballot(place > len - 1 - W);
+    if (lane == 0) {
+      flags[col / KB] = ((uint32_t)some ? 1u : 0u) | ((uint32_t)all == ~0u ? 2u : 0u);
+      flags[col / KB + 1] = ((uint32_t)(some >> 32) ? 1u : 0u) | ((uint32_t)(all >> 32) == ~0u ? 2u : 0u);
+    }
+  }
+  if (threadIdx.x < MOST) {
+    const int i = min((int)threadIdx.x, len - 1);
+    kp[W_MAX + threadIdx.x] = depth_of(ro.masks, i);
+  }
+  __syncthreads();
+
+  // ---- the wave's key blocks ----
+  const float sl2 = p.scale * LOG2E;
+  float m[T], sum[T];
+  f32x4 O[T][2][8];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    m[t] = -INFINITY;
+    sum[t] = 0.f;
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) O[t][hh][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  const int step = KW * p.splits;
+  const auto next_block = [&](int b) {   // the wave's next block that a query may see
+    for (b += step; b < n_blocks; b += step)
+      if (b >= RB || (__builtin_amdgcn_readfirstlane(flags[b]) & 1u)) break;
+    return b;
+  };
+  u32x4 kr[2][D / 32];
+  const auto load_keys = [&](int b) __attribute__((always_inline)) {
+    const bool ring = b < RB;
+    const uint16_t* base = ring ? ro.ring_k + b * (KB * D) : ro.k + (int64_t)(b - RB) * KB * p.nk_sl;
+    const int64_t st = ring ? D : p.nk_sl;
+    const int last = ring ? KB - 1 : len - 1 - (b - RB) * KB;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const uint16_t* src = base + min(16 * kt + c, last) * st + 8 * g4;
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ++ks) kr[kt][ks] = load16(src + 32 * ks);
+    }
+  };
+  int b = tiles > 0 ? next_block(wk + KW * split - step) : n_blocks;
+  if (b < n_blocks) load_keys(b);
+  while (b < n_blocks) {
+    const bool ring = b < RB;
+    const bool full = ring && (__builtin_amdgcn_readfirstlane(flags[b]) & 2u);
+    // ---- values: dims 128 hh + 8 c .. + 7 of keys 16 (s / 4) + 4 g4 + s % 4 ----
+    u32x4 vr[2][8];
+    {
+      const uint16_t* base = ring ? ro.ring_v + b * (KB * D) : ro.v + (int64_t)(b - RB) * KB * p.nv_sl;
+      const int64_t st = ring ? D : p.nv_sl;
+      const int last = ring ? KB - 1 : len - 1 - (b - RB) * KB;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const uint16_t* src = base + min(16 * (s >> 2) + 4 * g4 + (s & 3), last) * st + 8 * c;
+        vr[0][s] = load16(src);
+        vr[1][s] = load16(src + 128);
+      }
+    }
+    // ---- scores ----
+    f32x4 S[T][2];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      S[t][0] = S[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      if (t >= tiles) continue;
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ++ks) {
+        bf16x8 qf;
+        if constexpr (Q_LDS) qf = as_bf16x8(lds.q[wq * T + t][ks][lane]);
+        else qf = qr[t][ks];
+        S[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[0][ks]), qf, S[t][0], 0, 0, 0);
+        S[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[1][ks]), qf, S[t][1], 0, 0, 0);
+      }
+    }
+    const int b_now = b;
+    b = next_block(b);
+    if (b < n_blocks) load_keys(b);
+    // ---- masks ----
+    i32x4 place[2];
+    if (!full) {
+      const int at = (ring ? b_now * KB : W_MAX + (b_now - RB) * KB) + 4 * g4;
+      place[0] = *reinterpret_cast<const i32x4*>(&kp[at]);
+      place[1] = *reinterpret_cast<const i32x4*>(&kp[at + 16]);
+      // a value that no query of the row sees may hold anything
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const int key = 16 * (s >> 2) + 4 * g4 + (s & 3);
+        const bool live = ring ? place[s >> 2][s & 3] > -W : (b_now - RB) * KB + key <= l_hi;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) vr[hh][s] = live ? vr[hh][s] : (u32x4){0u, 0u, 0u, 0u};
+      }
+    }
+    float top[T];
+    bool move = false;
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      top[t] = -INFINITY;
+      if (t >= tiles) continue;
+      const uint32_t bits = (uint32_t)(mask[t] >> (ring ? 0 : (b_now - RB) * KB)) >> (4 * g4);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float s = S[t][kt][r] * sl2;
+          if (!full) {
+            const bool ok = place[kt][r] > depth[t] - W && (ring || (bits >> (16 * kt + r) & 1u));
+            s = ok ? s : -INFINITY;
+          }
+          S[t][kt][r] = s;
+          top[t] = fmaxf(top[t], s);
+        }
+      top[t] = max_pair32(max_pair16(top[t]));
+      move |= top[t] > m[t] + SLACK;
+    }
+    if (__any(move)) {
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        if (t >= tiles) continue;
+        const float to = top[t] > m[t] + SLACK ? top[t] : m[t];
+        const float alpha = to == -INFINITY ? 1.f : exp2_fast(m[t] - to);
+        m[t] = to;
+        sum[t] *= alpha;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) O[t][hh][i] *= alpha;
+      }
+    }
+    bf16x8 pb[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const float base = m[t] == -INFINITY ? 0.f : m[t];
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p0 = exp2_fast(S[t][i >> 1][2 * (i & 1)] - base), p1 = exp2_fast(S[t][i >> 1][2 * (i & 1) + 1] - base);
+        sum[t] += p0 + p1;
+        w[i] = pack_bf16x2(p0, p1);
+      }
+      pb[t] = as_bf16x8(w);
+    }
+    // ---- O^T += V^T . P^T ----
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = __builtin_amdgcn_perm(vr[hh][2 * e + 1][i >> 1], vr[hh][2 * e][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          if (t >= tiles) continue;
+          O[t][hh][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(w), pb[t], O[t][hh][i], 0, 0, 0);
+        }
+      }
+  }
+
+  // ---- the waves' partial sums meet ----
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    sum[t] = add_xor32(add_xor16(sum[t]));
+    if (g4 == 0) {
+      ml[wave][t][c][0] = m[t];
+      ml[wave][t][c][1] = sum[t];
+    }
+  }
+  __syncthreads();   // (the queries in LDS are read no more, either)
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    float top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int w = 0; w < KW; ++w) top = fmaxf(top, ml[wq * KW + w][t][c][0]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < KW; ++w) total += exp2_fast(ml[wq * KW + w][t][c][0] - base) * ml[wq * KW + w][t][c][1];
+    const float mine = exp2_fast(m[t] - base);
+    if (t) __syncthreads();   // the tile before is read
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) lds.o[wave][8 * hh + i][lane] = O[t][hh][i] * mine;
+    __syncthreads();
+    // lane (g4, c) of product (hh, i), register r: query c, dim 128 hh + 32 g4 + 8 r + i
+    constexpr int R = 8 / KW;           // registers of the lane: with KW waves 1 of KW pieces of the 2 x 4
+    const int hh = wk * R / 4, r0 = wk * R % 4;
+    float y[8 * R];
+#pragma unroll
+    for (int e = 0; e < 8 * R; ++e) y[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < KW; ++w)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float* src = reinterpret_cast<const float*>(&lds.o[wq * KW + w][8 * hh + i][lane]) + r0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) y[8 * r + i] += src[r];
+      }
+    const int row = r_lo + 16 * t + c;
+    const int d0 = 128 * hh + 32 * g4 + 8 * r0;
+    if (row < M) {
+      if (p.splits == 1) {
+        const float inv = 1.0f / total;
+#pragma unroll
+        for (int e = 0; e < 8 * R; ++e) y[e] *= inv;
+        finish(p, ro, row, d0, y);
+      } else {
+        const int64_t at = ((int64_t)pair * p.splits + split) * ((int64_t)G * p.max_nodes) + row;
+        float* dst = p.part_o + at * D + d0;
+#pragma unroll
+        for (int e = 0; e < 8 * R; e += 4) *reinterpret_cast<f32x4*>(dst + e) = (f32x4){y[e], y[e + 1], y[e + 2], y[e + 3]};
+        if (wk == 0 && g4 == 0) {
+          p.part_ml[2 * at] = top;
+          p.part_ml[2 * at + 1] = total;
+        }
+      }
+    }
+  }
+}
+
+// Joins the splits' partial sums: 16 lanes a query row, 16 dims a lane
+__global__ __launch_bounds__(256) void tree_attn_join_kernel(const TreeAttnParams p) {
+  const int pair = blockIdx.x;
+  const int n = pair / p.hkv, h = pair - n * p.hkv;
+  TreeKeys ro;
+  if (!tree_keys(p, n, h, ro)) return;
+  const int row = blockIdx.y * 16 + (threadIdx.x >> 4), d0 = 16 * (threadIdx.x & 15);
+  if (row >= p.G * ro.len) return;
+  const int64_t stride = (int64_t)p.G * p.max_nodes;
+  const int64_t first = (int64_t)pair * p.splits * stride + row;
+  float top = -INFINITY, total = 0.f;
+  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[2 * (first + s * stride)]);
+  const float base = top == -INFINITY ? 0.f : top;
+  float y[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) y[e] = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float w = exp2_fast(p.part_ml[2 * (first + s * stride)] - base);
+    total += w * p.part_ml[2 * (first + s * stride) + 1];
+    const float* src = p.part_o + (first + s * stride) * D + d0;
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(src + e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[e + i] = __builtin_fmaf(w, v[i], y[e + i]);
+    }
+  }
+  const float inv = 1.0f / total;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) y[e] *= inv;
+  finish(p, ro, row, d0, y);
+}
+
+// The committed chain's keys and values into the ring (of a chain longer than the window its last W), 16 nodes a workgroup:
+// a thread's 16-byte pieces are loaded before any of them is stored
+__global__ __launch_bounds__(256) void tree_ring_write_kernel(const TreeAttnParams p) {
+  const int n = blockIdx.x / p.hkv, h = blockIdx.x - n * p.hkv;
+  const int64_t slot = p.slots[n], len = p.lens[n], off = p.offsets[n], start = p.starts[n], done64 = p.commits[n];
+  if ((slot < 0) | (slot >= p.ring_rows) | (len <= 0) | (len > p.max_nodes) | (done64 <= 0)) return;
+  const int done = (int)(done64 > len ? len : done64);
+  const int first = max(0, done - p.W);
+  const int64_t ring = ((slot * p.hkv + h) * (int64_t)(p.W + 1)) * D;
+  const int64_t start_col = ((start % p.W) + p.W) % p.W;
+  constexpr int EACH = 2;   // nodes of a thread: 8 nodes of 32 pieces at a time
+  const int d = 8 * (threadIdx.x & 31);
+  u32x4 k[EACH], v[EACH];
+  int node[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    node[e] = first + blockIdx.y * (8 * EACH) + 8 * e + (int)(threadIdx.x >> 5);
+    const int64_t t = off + min(node[e], done - 1);
+    k[e] = load16(p.new_k + t * p.nk_sl + h * p.nk_sh + d);
+    v[e] = load16(p.new_v + t * p.nv_sl + h * p.nv_sh + d);
+  }
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    if (node[e] >= done) continue;
+    const int64_t at = ring + ((start_col + node[e]) % p.W) * D + d;
+    *reinterpret_cast<u32x4*>(p.ring_k + at) = k[e];
+    *reinterpret_cast<u32x4*>(p.ring_v + at) = v[e];
+  }
+}
+
+// Query rows of a workgroup, and the ways its keys are split over its waves. From 65 query rows on two waves share a query
+// group, which halves what meets in LDS at the end.
+inline int rows_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+
+// Workgroups of a row's key blocks: few rows leave the chip (256 CUs) short of workgroups, and one CU moves only a few tens
+// of GB/s. 4 at most: then a wave has one ring block of a full window.
+inline int splits_of(int64_t n_rows, int64_t hkv, int64_t rows) {
+  const int64_t units = n_rows * hkv * ((rows + rows_of(rows) - 1) / rows_of(rows));
+  return units <= 64 ? 4 : units <= 128 ? 2 : 1;
+}
+
+inline size_t part_bytes(int64_t n_rows, int64_t hkv, int64_t rows, int splits) {
+  return splits == 1 ? 0 : (size_t)(n_rows * hkv * splits * rows) * (D + 2) * sizeof(float);
+}
+
+}  // namespace
+}  // namespace hsg
+
+extern "C" size_t hsg_tree_attention_workspace_bytes(int32_t n_rows, int32_t hkv, int32_t groups, int32_t max_nodes) {
+  using namespace hsg;
+  if (n_rows <= 0 || hkv <= 0 || groups <= 0 || max_nodes <= 0 || max_nodes > MOST) return 0;
+  const int64_t rows = (int64_t)groups * max_nodes;
+  return part_bytes(n_rows, hkv, rows, splits_of(n_rows, hkv, rows));
+}
+
+extern "C" int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int64_t q_sg, void* ring_k, void* ring_v,
+                                  int64_t ring_rows, int32_t window, const void* new_k, int64_t nk_sl, int64_t nk_sh,
+                                  const void* new_v, int64_t nv_sl, int64_t nv_sh, const void* gate, int64_t g_sl,
+                                  int64_t g_sh, int64_t g_sg, int64_t g_off, const int64_t* ring_pos,
+                                  const int64_t* slots, const int64_t* starts, const int64_t* lens,
+                                  const int64_t* offsets, const int64_t* commits, const int64_t* masks, int32_t n_rows,
+                                  int32_t max_nodes, int32_t hkv, int32_t groups, int32_t head_dim, float scale, void* out,
+                                  int64_t o_sl, int64_t o_sh, int64_t o_sg, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  using namespace hsg;
+  if (n_rows < 0 || hkv <= 0 || groups <= 0 || ring_rows <= 0) return HSG_ERR_ARG;
+  if (head_dim != D || window <= 0 || window > W_MAX || window % KB != 0 || max_nodes <= 0 || max_nodes > MOST)
+    return HSG_ERR_SHAPE;
+  if (n_rows == 0) return HSG_OK;
+  if (!q || !ring_k || !ring_v || !new_k || !new_v || !ring_pos || !slots || !starts || !lens || !offsets || !masks || !out)
+    return HSG_ERR_ARG;
+  const int64_t strides[] = {q_sl, q_sh, q_sg, nk_sl, nk_sh, nv_sl, nv_sh, o_sl, o_sh, o_sg};
+  for (int64_t st : strides)
+    if (st % 8) return HSG_ERR_ALIGN;
+  if (gate && (g_sl % 8 || g_sh % 8 || g_sg % 8 || g_off % 8 || !aligned(gate, 16))) return HSG_ERR_ALIGN;
+  if (!aligned(q, 16) || !aligned(ring_k, 16) || !aligned(ring_v, 16) || !aligned(new_k, 16) || !aligned(new_v, 16) ||
+      !aligned(out, 16) || !aligned(workspace, 16))
+    return HSG_ERR_ALIGN;
+  const int64_t rows = (int64_t)groups * max_nodes;
+  const int64_t pairs = (int64_t)n_rows * hkv;
+  const int per_wg = rows_of(rows);
+  TreeAttnParams p{};
+  p.q = static_cast<const uint16_t*>(q); p.q_sl = q_sl; p.q_sh = q_sh; p.q_sg = q_sg;
+  p.ring_k = static_cast<uint16_t*>(ring_k); p.ring_v = static_cast<uint16_t*>(ring_v);
+  p.ring_rows = ring_rows; p.W = window;
+  p.new_k = static_cast<const uint16_t*>(new_k); p.nk_sl = nk_sl; p.nk_sh = nk_sh;
+  p.new_v = static_cast<const uint16_t*>(new_v); p.nv_sl = nv_sl; p.nv_sh = nv_sh;
+  p.gate = static_cast<const uint16_t*>(gate); p.g_sl = g_sl; p.g_sh = g_sh; p.g_sg = g_sg; p.g_off = g_off;
+  p.ring_pos = ring_pos; p.slots = slots; p.starts = starts; p.lens = lens; p.offsets = offsets;
+  p.commits = commits; p.masks = masks;
+  p.max_nodes = max_nodes; p.hkv = hkv; p.G = groups; p.scale = scale;
+  if (pairs >= (1 << 24) || rows >= (1 << 20)) return HSG_ERR_SHAPE;
+  p.pairs = (int)pairs;
+  p.qblocks = (int)((rows + per_wg - 1) / per_wg);
+  p.splits = splits_of(n_rows, hkv, rows);
+  if (!workspace || workspace_bytes < part_bytes(n_rows, hkv, rows, p.splits)) p.splits = 1;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.splits > 1 ? p.part_o + pairs * p.splits * rows * D : nullptr;
+  p.out = static_cast<uint16_t*>(out); p.o_sl = o_sl; p.o_sh = o_sh; p.o_sg = o_sg;
+  const int64_t blocks = (pairs + 7) / 8 * 8 * p.qblocks * p.splits;
+  if (blocks >= (1 << 24)) return HSG_ERR_SHAPE;   // a launch holds less than 2^32 threads
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NW), 0, st, p); };
+  if (per_wg == 16) launch(tree_attn_kernel<1, 4>);
+  else if (per_wg == 32) launch(tree_attn_kernel<2, 4>);
+  else if (per_wg == 64) launch(tree_attn_kernel<4, 4>);
+  else launch(tree_attn_kernel<4, 2>);
+  if (p.splits > 1)
+    hipLaunchKernelGGL(tree_attn_join_kernel, dim3((unsigned)pairs, (unsigned)((rows + 15) / 16)), dim3(256), 0, st, p);
+  if (commits)
+    hipLaunchKernelGGL(tree_ring_write_kernel, dim3((unsigned)pairs, (unsigned)((max_nodes + 15) / 16)), dim3(256), 0, st, p);
+  return launch_status();
+}

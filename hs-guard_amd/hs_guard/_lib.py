@@ -20,6 +20,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libhsg.so")
 HSG_OK, HSG_ERR_ARG, HSG_ERR_ALIGN, HSG_ERR_SHAPE, HSG_ERR_BLAS = 0, -1, -2, -3, -4
 HSG_GDN_BURST_MIN_DEFAULT = 16   # include/hsg.h
 HSG_GEMM_SKINNY_M_MAX = 8        # include/hsg.h
+HSG_TREE_MAX_NODES = 64          # include/hsg.h
 
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -154,6 +155,30 @@ SIGNATURES = {
                                                     _I32, _I32, _P, _P]),
     "hsg_gemm_candidates": (ctypes.c_int, [_I32, _I32, _I32, _P, _P, _I32, ctypes.c_size_t]),
     "hsg_gemm_blas_version": (ctypes.c_int, []),
+    "hsg_tree_maps": (ctypes.c_int, [
+        _P, _I64, _P, _P, _P, _I32, _I32,    # parents, tokens, lens, starts, commits, n_rows, max_nodes
+        _P, _P, _P, _P, _P, _P]),            # offsets, lens_out, commits_out, pos, masks, stream
+    "hsg_tree_conv_silu": (ctypes.c_int, [
+        _P, _I64, _P, _I64, _P, _I32,        # x, x_stride, pool, pool_rows, weight, kernel_size
+        _P, _P, _P, _P, _P, _I32, _I32,      # slots, lens, offsets, commits, masks, n_rows, max_nodes
+        _I32, _P, _I64, _P]),                # channels, out, out_stride, stream
+    "hsg_gdn_tree_step": (ctypes.c_int, [
+        _P, _I64, _I32, _I32, _I32,          # qkv, qkv_stride, q_off, k_off, v_off
+        _P, _P, _I64, _P, _P,                # a, b, ab_stride, A_log, dt_bias
+        _P, _I32, _I64,                      # state, state_dtype, state_rows
+        _P, _P, _P, _P, _P, _I32, _I32,      # slots, lens, offsets, commits, masks, n_rows, max_nodes
+        _I32, _I32, _I32, _I32, _F,          # H, HV, K, V, scale
+        _P, _I64, _P, _F, _P, _P]),          # z, z_stride, norm_w, eps, out, stream
+    "hsg_tree_attention_workspace_bytes": (ctypes.c_size_t, [_I32, _I32, _I32, _I32]),
+    "hsg_tree_attention": (ctypes.c_int, [
+        _P, _I64, _I64, _I64,                # q, q_sl, q_sh, q_sg
+        _P, _P, _I64, _I32,                  # ring_k, ring_v, ring_rows, window
+        _P, _I64, _I64, _P, _I64, _I64,      # new_k, nk_sl, nk_sh, new_v, nv_sl, nv_sh
+        _P, _I64, _I64, _I64, _I64,          # gate, g_sl, g_sh, g_sg, g_off
+        _P, _P, _P, _P, _P, _P, _P,          # ring_pos, slots, starts, lens, offsets, commits, masks
+        _I32, _I32, _I32, _I32, _I32, _F,    # n_rows, max_nodes, hkv, groups, head_dim, scale
+        _P, _I64, _I64, _I64,                # out, o_sl, o_sh, o_sg
+        _P, ctypes.c_size_t, _P]),           # workspace, workspace_bytes, stream
 }
 
 _lib = None

@@ -7,9 +7,11 @@ called under hipGraph capture. There is no fallback: a missing library raises Ru
 """
 from __future__ import annotations
 
+from typing import NamedTuple, Optional
+
 import torch
 
-from .._lib import HSG_GDN_BURST_MIN_DEFAULT, calls, check, lib
+from .._lib import HSG_GDN_BURST_MIN_DEFAULT, HSG_TREE_MAX_NODES, calls, check, lib
 
 HSG_STATE_F32 = 0
 HSG_STATE_F16 = 1
@@ -318,4 +320,191 @@ def ring_attention(q, ring_k, ring_v, new_k, new_v, ring_pos, slots, starts, len
         n, lb, hkv, groups, d, float(scale), 0, 0,
         _ptr(out), hkv * m * d, d, m * d, lb * d, _stream(q))
     check(rc, "hsg_ring_attention")
+    return out
+
+
+# ------------------------------------------------------------------------------------------------------------
+# Drafted trees (no counterpart in the reference): candidate tokens of live sessions, scored against their state without
+# moving it; a row's first nodes, a chain, can be committed in the same call
+# ------------------------------------------------------------------------------------------------------------
+class DraftTrees(NamedTuple):
+    """A packed batch of trees (``draft_tree_maps``): row n's nodes are tokens offsets[n] .. offsets[n] + lens[n] - 1,
+    parents first. Rows with ``lens`` 0 have no nodes."""
+    offsets: torch.Tensor               # [n] int64
+    lens: torch.Tensor                  # [n] int64
+    commits: Optional[torch.Tensor]     # [n] int64: leading nodes that move the session's state; None: nothing moves
+    pos: torch.Tensor                   # [T] int64: start + depth
+    masks: torch.Tensor                 # [T] int64 of 64 bits: the node's ancestors and itself, by their index in the row
+    max_nodes: int = HSG_TREE_MAX_NODES     # bound on every row's nodes; smaller bounds take smaller tiles
+
+
+def _index_tensors(like, *tensors):
+    """The index tensors (None skipped) are contiguous int64 on the device of ``like``."""
+    for t in tensors:
+        _require(t is None or (t.dtype is torch.int64 and t.is_contiguous() and t.device == like.device),
+                 "index tensors must be contiguous int64 on the operands' device")
+
+
+def _tree_rows(trees, slots, tokens, like):
+    """Checks of a batch of trees over ``tokens`` packed tokens; returns its rows."""
+    n = slots.shape[0]
+    _index_tensors(like, slots, *trees[:5])
+    _require(slots.dim() == 1 and trees.offsets.shape == (n,) and trees.lens.shape == (n,)
+             and (trees.commits is None or trees.commits.shape == (n,)), "offsets, lens, commits and slots must be [n]")
+    _require(trees.masks.shape == (tokens,), "masks must be [T], one for each packed token")
+    _require(1 <= trees.max_nodes <= HSG_TREE_MAX_NODES, f"max_nodes must be in [1, {HSG_TREE_MAX_NODES}]")
+    return n
+
+
+def _packed_rows(t, width):
+    """t's rows [T, ...] lie ``stride(0)`` apart, each one's ``width`` values next to one another."""
+    _require(t.dtype is torch.bfloat16, "bf16 tensors expected")
+    inner = 1
+    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        _require(size == 1 or stride == inner, "a token's values must be contiguous")
+        inner *= size
+    _require(inner == width, f"{width} values a token expected, got {inner}")
+    _require(t.shape[0] <= 1 or t.stride(0) >= width, "tokens must not overlap")
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
+class _on:
+    """The device of ``t`` as the current one: a launch goes to the current device, whatever its stream."""
+
+    def __init__(self, t):
+        self.device = t.device.index
+
+    def __enter__(self):
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.device:
+            torch._C._cuda_setDevice(self.device)
+
+    def __exit__(self, *exc):
+        if self.before != self.device:
+            torch._C._cuda_setDevice(self.before)
+
+
+def draft_tree_maps(parents, lens, starts, commits=None, max_nodes=HSG_TREE_MAX_NODES):
+    """The maps of a packed batch of drafted trees, built on the GPU: ``DraftTrees``. parents [T] int64: each node's parent
+    by its index in the row (-1: a child of the session's last token), rows one after another; lens, starts, commits [n]
+    int64: nodes of each row, tokens its session holds, leading nodes to commit. A row that is no tree (a parent that does
+    not come before its child, more than ``max_nodes`` nodes or more than the buffer holds, commits that are no chain from
+    the session's last token) comes back with lens and commits 0. pos and masks of tokens of no row are 0."""
+    _gpu(parents, lens, starts, commits)
+    _index_tensors(parents, parents, lens, starts, commits)
+    n = lens.shape[0]
+    _require(parents.dim() == 1 and lens.dim() == 1 and starts.shape == (n,) and (commits is None or commits.shape == (n,)),
+             "parents must be [T]; lens, starts and commits [n]")
+    _require(1 <= max_nodes <= HSG_TREE_MAX_NODES, f"max_nodes must be in [1, {HSG_TREE_MAX_NODES}]")
+    total = parents.shape[0]
+    offsets, lens_out = torch.empty_like(lens), torch.empty_like(lens)
+    commits_out = None if commits is None else torch.empty_like(commits)
+    pos, masks = torch.empty_like(parents), torch.empty_like(parents)
+    with _on(parents):
+        rc = calls().hsg_tree_maps(_ptr(parents), total, _ptr(lens), _ptr(starts), _ptr(commits), n, max_nodes,
+                                   _ptr(offsets), _ptr(lens_out), _ptr(commits_out), _ptr(pos), _ptr(masks),
+                                   _stream(parents))
+    check(rc, "hsg_tree_maps")
+    return DraftTrees(offsets, lens_out, commits_out, pos, masks, max_nodes)
+
+
+def tree_conv_silu(qkv, pool, weight, slots, trees):
+    """silu(causal depthwise conv) of each node along its own path, past the root over the slot's history: qkv [T, C] bf16
+    (rows may lie further apart), pool [S, 3, C] bf16 (one layer), weight [C, 1, 4] bf16. Returns [T, C] bf16; tokens of no
+    row are not written. Rows that commit move their history in ``pool`` and need slots of their own."""
+    total, c = qkv.shape
+    _gpu(qkv, pool, weight, slots)
+    stride = _packed_rows(qkv, c)
+    _bf16_in(pool, weight)
+    ks = weight.shape[-1]
+    _require(pool.dim() == 3 and pool.shape[1:] == (ks - 1, c) and weight.numel() == c * ks,
+             "tree_conv_silu: pool [S, K-1, C], weight [C, 1, K]")
+    n = _tree_rows(trees, slots, total, qkv)
+    out = torch.empty((total, c), dtype=qkv.dtype, device=qkv.device)
+    with _on(qkv):
+        rc = calls().hsg_tree_conv_silu(_ptr(qkv), stride, _ptr(pool), pool.shape[0], _ptr(weight), ks, _ptr(slots),
+                                        _ptr(trees.lens), _ptr(trees.offsets), _ptr(trees.commits), _ptr(trees.masks), n,
+                                        trees.max_nodes, c, _ptr(out), c, _stream(qkv))
+    check(rc, "hsg_tree_conv_silu")
+    return out
+
+
+def gdn_tree_step(packed, key_dim, heads, head_k, value_heads, head_v, a, b, A_log, dt_bias, state, slots, trees,
+                  scale=None, z=None, norm_weight=None, eps=1e-6):
+    """The gated-delta rule along each node's path from state[slots[n]] (gdn_slot_v8's recurrence; every branch goes on from
+    its parent's state): packed [T, 2*key_dim + HV*V] bf16 (tree_conv_silu's output), a, b [T, HV] bf16, A_log, dt_bias [HV]
+    bf16, state [S, HV, K, V] fp32 or fp16. With z [T, HV*V] bf16 the layer's gated RMSNorm is applied (norm_weight [V]
+    bf16); a, b and z may be columns of a wider projection. Returns [T, HV*V] bf16; tokens of no row are not written. Rows
+    that commit move their state and need slots of their own; no other state is written."""
+    total = packed.shape[0]
+    hvv = value_heads * head_v
+    _gpu(packed, a, b, A_log, dt_bias, state, slots, z, norm_weight)
+    stride = _packed_rows(packed, 2 * key_dim + hvv)
+    _require(key_dim == heads * head_k, "key_dim must be heads * head_k")
+    _require(a.shape == (total, value_heads) and b.shape == a.shape, "a and b must be [T, HV]")
+    ab = _packed_rows(a, value_heads)
+    _require(_packed_rows(b, value_heads) == ab, "a and b must have one row stride")
+    _bf16_in(A_log, dt_bias)
+    _require(A_log.numel() == value_heads and dt_bias.numel() == value_heads, "A_log and dt_bias must be [HV]")
+    _require(state.dtype in _STATE_CODES and state.is_contiguous() and state.shape[1:] == (value_heads, head_k, head_v),
+             "state must be contiguous [S, HV, K, V], float32 or float16")
+    _require((z is None) == (norm_weight is None), "the gated norm takes z and norm_weight")
+    z_stride = 0
+    if z is not None:
+        _require(z.shape[0] == total, "z must be [T, HV*V]")
+        z_stride = _packed_rows(z, hvv)
+        _bf16_in(norm_weight)
+        _require(norm_weight.numel() == head_v, "norm_weight must be [V]")
+    n = _tree_rows(trees, slots, total, packed)
+    out = torch.empty((total, hvv), dtype=packed.dtype, device=packed.device)
+    scale = head_k ** -0.5 if scale is None else scale
+    with _on(packed):
+        rc = calls().hsg_gdn_tree_step(
+            _ptr(packed), stride, 0, key_dim, 2 * key_dim, _ptr(a), _ptr(b), ab, _ptr(A_log), _ptr(dt_bias), _ptr(state),
+            _STATE_CODES[state.dtype], state.shape[0], _ptr(slots), _ptr(trees.lens), _ptr(trees.offsets),
+            _ptr(trees.commits), _ptr(trees.masks), n, trees.max_nodes, heads, value_heads, head_k, head_v, float(scale),
+            _ptr(z), z_stride, _ptr(norm_weight), float(eps), _ptr(out), _stream(packed))
+    check(rc, "hsg_gdn_tree_step")
+    return out
+
+
+def tree_ring_attention(q, ring_k, ring_v, new_k, value, gate, ring_pos, slots, starts, trees, scale, window,
+                        workspace=None):
+    """Window attention of each node over its slot's ring (the keys before starts[n]) and its own ancestors, gated: q
+    [T, Hq, D], new_k and value [T, Hkv, D] bf16 (tokens may lie further apart), gate: q_proj output [T, Hq*2D] (gate =
+    second half of each head) or None, ring_k / ring_v [S, Hkv, W+1, D] bf16, ring_pos [S, W+1] int64. Returns
+    softmax(..) v * sigmoid(gate) as [T, Hq*D] bf16; tokens of no row are not written. Rows that commit write their chain's
+    keys and values into the ring (ring_pos stays the caller's) and need slots of their own. workspace: a uint8 device
+    tensor of hsg_tree_attention_workspace_bytes, which calls of few rows use (allocated per call when None)."""
+    total, hq, d = q.shape
+    hkv = new_k.shape[1]
+    _gpu(q, ring_k, ring_v, new_k, value, gate, ring_pos, slots, starts, workspace)
+    _require(hkv > 0 and hq % hkv == 0, "query heads must be a multiple of the kv heads")
+    groups = hq // hkv
+    _require(new_k.shape == (total, hkv, d) and value.numel() == total * hkv * d and value.shape[0] == total,
+             "new_k and value must be [T, Hkv, D]")
+    qs, ks, vs = _packed_rows(q, hq * d), _packed_rows(new_k, hkv * d), _packed_rows(value, hkv * d)
+    gs = 0
+    if gate is not None:
+        _require(gate.shape[0] == total, "gate must be [T, Hq*2D]")
+        gs = _packed_rows(gate, hq * 2 * d)
+    _bf16_in(ring_k, ring_v)
+    _require(ring_k.dim() == 4 and ring_k.shape[1:] == (hkv, window + 1, d) and ring_v.shape == ring_k.shape,
+             "ring_k and ring_v must be [S, Hkv, W+1, D]")
+    _require(ring_pos.shape == (ring_k.shape[0], window + 1), "ring_pos must be [S, W+1]")
+    _index_tensors(q, ring_pos, starts)
+    n = _tree_rows(trees, slots, total, q)
+    _require(starts.shape == (n,), "starts must be [n]")
+    out = torch.empty((total, hq * d), dtype=q.dtype, device=q.device)
+    if workspace is None:
+        need = lib().hsg_tree_attention_workspace_bytes(n, hkv, groups, trees.max_nodes)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    with _on(q):
+        rc = calls().hsg_tree_attention(
+            _ptr(q), qs, groups * d, d, _ptr(ring_k), _ptr(ring_v), ring_k.shape[0], window, _ptr(new_k), ks, d,
+            _ptr(value), vs, d, _ptr(gate), gs, groups * 2 * d, 2 * d, d, _ptr(ring_pos), _ptr(slots), _ptr(starts),
+            _ptr(trees.lens), _ptr(trees.offsets), _ptr(trees.commits), _ptr(trees.masks), n, trees.max_nodes, hkv, groups,
+            d, float(scale), _ptr(out), hq * d, groups * d, d, _ptr(workspace), 0 if workspace is None else
+            workspace.numel(), _stream(q))
+    check(rc, "hsg_tree_attention")
     return out

@@ -515,6 +515,82 @@ int hsg_gemm_bf16_skinny_addnorm(const void* hidden, int64_t ldh, const void* mi
 /* hipBLASLt's version on the current device (solution indices are valid only for the version they came from). */
 int hsg_gemm_blas_version(void);
 
+/*
+ * Drafted trees over live sessions (no counterpart in the reference): a tree of candidate tokens of a session is scored
+ * against the session's state without moving it; a row's first commits[n] nodes, a chain, are accepted and move it as a
+ * step would. Packed rows: row n's nodes are tokens offsets[n] .. offsets[n] + lens[n] - 1, in an order in which every
+ * parent comes before its children, at most HSG_TREE_MAX_NODES of them. masks[t] (int64 holding 64 bits): bit j is set for
+ * node j of the row if it is token t's node itself or one of its ancestors. Rows with lens[n] <= 0 or > max_nodes, or a
+ * slot outside the pool, are left alone, as are tokens of no row. Rows that commit need slots of their own in the call;
+ * rows that do not may share one. commits may be NULL: nothing moves.
+ */
+#define HSG_TREE_MAX_NODES 64
+
+/*
+ * The maps of a packed batch of trees, from the rows' lengths and the nodes' parents (row-local; -1: a child of the
+ * session's last token):
+ *   offsets[n] = sum of the lengths before n (negative ones count 0);  lens_out[n], commits_out[n] = lens[n], commits[n],
+ *   or 0 for a row that is no tree (a parent not in [-1, node), more than max_nodes nodes or more than the buffer holds, a
+ *   negative start, commits outside [0, lens[n]] or over nodes that are no chain);  pos[t] = starts[n] + depth (the roots'
+ *   is 0);  masks[t] as above; pos and masks of tokens of no row are 0.
+ *   parents, pos, masks [tokens] int64; lens, starts, commits, offsets, lens_out, commits_out [n_rows] int64 (commits and
+ *   commits_out may be NULL). The outputs must not overlap the inputs. One launch. Supported: max_nodes <= 64.
+ */
+int hsg_tree_maps(const int64_t* parents, int64_t tokens, const int64_t* lens, const int64_t* starts,
+                  const int64_t* commits, int32_t n_rows, int32_t max_nodes, int64_t* offsets, int64_t* lens_out,
+                  int64_t* commits_out, int64_t* pos, int64_t* masks, void* stream);
+
+/*
+ * Causal depthwise conv + SiLU along each node's path: the values of the node and of its three nearest ancestors, past the
+ * root those of the slot's history.
+ *   x [tokens, x_stride] bf16 (first `channels` columns), pool [pool_rows, 3, channels] bf16, oldest first, weight
+ *   [channels, 4] bf16, out [tokens, out_stride] bf16, summed in fp32 and rounded once. Rows with commits[n] > 0 move the
+ *   history by their chain. out may be x itself with the same stride; otherwise the two must not overlap.
+ * Supported: kernel_size == 4, at most 65,535 rows; channels and strides multiples of 8, pointers 16-byte aligned.
+ */
+int hsg_tree_conv_silu(const void* x, int64_t x_stride, void* pool, int64_t pool_rows, const void* weight,
+                       int32_t kernel_size, const int64_t* slots, const int64_t* lens, const int64_t* offsets,
+                       const int64_t* commits, const int64_t* masks, int32_t n_rows, int32_t max_nodes,
+                       int32_t channels, void* out, int64_t out_stride, void* stream);
+
+/*
+ * The gated-delta rule along each node's path from the slot's state (hsg_gdn_slot_step's recurrence, every branch from the
+ * state that its parent leaves), and the layer's gated RMSNorm:
+ *   z != NULL: out[t, hv*V + c] = bf16(norm_w[c] * o * rsqrt(mean(o^2) + eps) * silu(z[t, hv*V + c])), rounded once;
+ *   z == NULL: out = bf16(o), and norm_w and eps are not read.
+ *   qkv, a, b, A_log, dt_bias, state, z, norm_w, out as hsg_gdn_slot_step_gated's. Rows with commits[n] > 0 move the state
+ *   by their chain; no other state is written. A NaN or an infinity reaches its node and that node's descendants alone.
+ * Supported: K == V == 128, HV % H == 0; qkv and its offsets and stride 16-byte aligned.
+ */
+int hsg_gdn_tree_step(const void* qkv, int64_t qkv_stride, int32_t q_off, int32_t k_off, int32_t v_off, const void* a,
+                      const void* b, int64_t ab_stride, const void* A_log, const void* dt_bias, void* state,
+                      int32_t state_dtype, int64_t state_rows, const int64_t* slots, const int64_t* lens,
+                      const int64_t* offsets, const int64_t* commits, const int64_t* masks, int32_t n_rows,
+                      int32_t max_nodes, int32_t H, int32_t HV, int32_t K, int32_t V, float scale, const void* z,
+                      int64_t z_stride, const void* norm_w, float eps, void* out, void* stream);
+
+/*
+ * Window attention of the trees' nodes: node i of row n, at position starts[n] + depth, sees the slot's ring columns with
+ * 0 <= ring_pos < starts[n] and ring_pos > position - window, and of the row's own keys its ancestors' and its own with
+ * position - window < theirs. out = bf16(softmax(scale q.k) . v * sigmoid(gate)), rounded once; probabilities are rounded to
+ * bf16 for their product. gate may be NULL: no gating. Element addresses, ring pools and ring_pos as hsg_ring_attention's
+ * packed layout. Rows with commits[n] > 0 write their chain's keys and values into the ring columns (starts[n] + j) % window
+ * (of a chain longer than the window the last `window`), in a launch after the reads; ring_pos is the caller's
+ * (hsg_ring_pos_update with lens = commits). A NaN or an infinity reaches only the nodes that see it.
+ * workspace (optional): with at least hsg_tree_attention_workspace_bytes(n_rows, hkv, groups, max_nodes) bytes (0: none is
+ * used), 16-byte aligned, calls of few rows split a row's keys over workgroups; its contents need no initialisation.
+ * Supported: head_dim == 256, window <= 512 and a multiple of 32; strides multiples of 8, pointers 16-byte aligned.
+ */
+size_t hsg_tree_attention_workspace_bytes(int32_t n_rows, int32_t hkv, int32_t groups, int32_t max_nodes);
+int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int64_t q_sg, void* ring_k, void* ring_v,
+                       int64_t ring_rows, int32_t window, const void* new_k, int64_t nk_sl, int64_t nk_sh,
+                       const void* new_v, int64_t nv_sl, int64_t nv_sh, const void* gate, int64_t g_sl, int64_t g_sh,
+                       int64_t g_sg, int64_t g_off, const int64_t* ring_pos, const int64_t* slots,
+                       const int64_t* starts, const int64_t* lens, const int64_t* offsets, const int64_t* commits,
+                       const int64_t* masks, int32_t n_rows, int32_t max_nodes, int32_t hkv, int32_t groups,
+                       int32_t head_dim, float scale, void* out, int64_t o_sl, int64_t o_sh, int64_t o_sg,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

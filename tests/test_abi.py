@@ -161,3 +161,66 @@ def test_contract_glue_refuses_more_threads_than_a_launch_holds():
     L = lib()
     assert L.hsg_silu_mul_pair(2, 2, 2, 1 << 32, None) == HSG_ERR_SHAPE
     assert L.hsg_add_square(2, 2, 2, 4, 1 << 20, 1 << 12, None) == HSG_ERR_SHAPE
+
+
+def test_tree_operators_refuse_before_launch():
+    """Sizes, strides and pointers that the tree kernels do not take (placeholder pointers, never read)."""
+    from hs_guard import _lib
+    L = _lib.lib()
+    text = open(HEADER).read()
+    assert int(re.search(r"#define HSG_TREE_MAX_NODES (\d+)", text).group(1)) == _lib.HSG_TREE_MAX_NODES
+    ARG, ALIGN, SHAPE = _lib.HSG_ERR_ARG, _lib.HSG_ERR_ALIGN, _lib.HSG_ERR_SHAPE
+
+    def maps(*, parents=256, tokens=8, lens=256, starts=256, commits=256, rows=2, most=64, offsets=512, lens_out=768,
+             commits_out=1024, pos=1280, masks=1536):
+        return L.hsg_tree_maps(parents, tokens, lens, starts, commits, rows, most, offsets, lens_out, commits_out, pos,
+                               masks, None)
+
+    assert maps(rows=0, tokens=0) == 0
+    assert [maps(most=m) for m in (0, 65)] == [SHAPE, SHAPE]
+    for bad in ({"rows": -1}, {"tokens": -1}, {"parents": None}, {"lens": None}, {"starts": None}, {"commits_out": None},
+                {"lens_out": 256}, {"offsets": 256}, {"pos": None}, {"masks": None}):
+        assert maps(**bad) == ARG, bad
+
+    def conv(*, x=256, stride=64, pool=256, pool_rows=2, weight=256, ks=4, lens=256, masks=256, rows=2, most=64,
+             channels=64, out=512, out_stride=64):
+        return L.hsg_tree_conv_silu(x, stride, pool, pool_rows, weight, ks, 256, lens, 256, None, masks, rows, most,
+                                    channels, out, out_stride, None)
+
+    assert conv(rows=0) == 0
+    for bad, rc in (({"ks": 3}, SHAPE), ({"most": 65}, SHAPE), ({"most": 0}, SHAPE), ({"rows": 65536}, SHAPE),
+                    ({"pool_rows": 0}, ARG), ({"channels": 0}, ARG), ({"pool": None}, ARG), ({"masks": None}, ARG),
+                    ({"stride": 56}, ARG), ({"out_stride": 56}, ARG), ({"out": 256, "out_stride": 72}, ARG),
+                    ({"channels": 60}, ALIGN), ({"stride": 68}, ALIGN), ({"x": 264}, ALIGN), ({"out": 520}, ALIGN)):
+        assert conv(**bad) == rc, bad
+
+    def step(*, qkv=256, stride=512, a=256, state=256, dtype=0, state_rows=2, masks=256, rows=2, most=64, H=1, HV=1, K=128,
+             V=128, z=256, z_stride=128, norm=256, out=512, off=0, ab=1):
+        return L.hsg_gdn_tree_step(qkv, stride, off, 128, 256, a, 256, ab, 256, 256, state, dtype, state_rows, 256, 256,
+                                   256, None, masks, rows, most, H, HV, K, V, 1.0, z, z_stride, norm, 1e-6, out, None)
+
+    assert step(rows=0) == 0
+    for bad, rc in (({"K": 64}, SHAPE), ({"V": 64}, SHAPE), ({"most": 65}, SHAPE), ({"rows": 1 << 24}, SHAPE),
+                    ({"HV": 3, "H": 2}, ARG), ({"dtype": 2}, ARG), ({"a": None}, ARG), ({"masks": None}, ARG),
+                    ({"norm": None}, ARG), ({"z_stride": 64}, ARG), ({"ab": 0}, ARG), ({"off": -8}, ARG),
+                    ({"state_rows": 0}, ARG), ({"stride": 516}, ALIGN), ({"off": 4}, ALIGN), ({"state": 264}, ALIGN),
+                    ({"z": 258}, ALIGN), ({"out": 514}, ALIGN)):
+        assert step(**bad) == rc, bad
+
+    def attend(*, q=256, q_sl=512, ring_k=256, ring_rows=2, window=512, k_sl=256, gate=256, g_sl=1024, ring_pos=256,
+               masks=256, rows=2, most=64, hkv=1, G=2, dim=256, out=512, o_sl=512, ws=None, ws_bytes=0):
+        return L.hsg_tree_attention(q, q_sl, 512, 256, ring_k, 256, ring_rows, window, 256, k_sl, 256, 256, 256, 256, gate,
+                                    g_sl, 1024, 512, 256, ring_pos, 256, 256, 256, 256, None, masks, rows, most, hkv, G,
+                                    dim, 1.0, out, o_sl, 512, 256, ws, ws_bytes, None)
+
+    assert attend(rows=0) == 0
+    for bad, rc in (({"dim": 128}, SHAPE), ({"window": 544}, SHAPE), ({"window": 40}, SHAPE), ({"most": 65}, SHAPE),
+                    ({"rows": 1 << 24}, SHAPE), ({"hkv": 0}, ARG), ({"G": 0}, ARG), ({"ring_rows": 0}, ARG),
+                    ({"q": None}, ARG), ({"ring_pos": None}, ARG), ({"masks": None}, ARG), ({"q_sl": 516}, ALIGN),
+                    ({"k_sl": 260}, ALIGN), ({"g_sl": 1028}, ALIGN), ({"q": 264}, ALIGN), ({"out": 520}, ALIGN),
+                    ({"ws": 264, "ws_bytes": 1 << 30}, ALIGN)):
+        assert attend(**bad) == rc, bad
+    need = L.hsg_tree_attention_workspace_bytes
+    assert need(1, 4, 4, 12) == 4 * 4 * 48 * 258 * 4      # 4 kv heads, 4 splits, 48 query rows of 256 sums, maximum, weight
+    assert need(20, 4, 4, 12) == 20 * 4 * 2 * 48 * 258 * 4
+    assert need(352, 4, 4, 12) == 0 and need(0, 4, 4, 12) == 0 and need(1, 4, 4, 65) == 0
