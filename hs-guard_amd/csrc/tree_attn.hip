@@ -4,23 +4,30 @@
 // tree's keys those of its ancestors and its own that lie within W of it. Nothing of the ring moves but, in a second launch
 // after all reads, the columns of the committed chain.
 //
-// Query rows r = node * G + (query head of the kv head) form tiles of 16. A workgroup of 4 waves takes one (row, kv head) and
-// 16 T QW query rows, as QW x KW waves (QW KW = 4): the KW waves of a query group split the KEYS, blocks of 32 in turn, so a
-// wave's keys and values go straight from memory to its operand registers, each read once for its T tiles, with no LDS, no
-// barrier and no wave waiting for another in the loop. Per block, on v_mfma_f32_16x16x32_bf16:
+// Query rows r = node * G + (query head of the kv head) form tiles of 16, 1 or 2 to a wave. Per block of 32 keys, on
+// v_mfma_f32_16x16x32_bf16:
 //   S^T[key, query] = K . Q^T      a lane's column is one query: maxima, sums and rescales are per-lane scalars
 //   O^T[d, query] += V^T . P^T     B = P straight from the S^T accumulators (the product's key order is the lane's own);
 //                                  A = V^T: a lane reads 8 dims of its 8 keys and swaps 16-bit halves in registers, product
 //                                  i of 8 taking dim 8 c + i of each lane c
 // The running maximum is moved only when a block's exceeds it by 2^8, so the accumulators are seldom rescaled; sums are fp32
-// and P is rounded to bf16 for its product (2^-9 of each weight, below the output's own rounding). At the end the waves'
-// partial sums meet in LDS, weighted by their maxima. Where few rows leave the chip short of workgroups, NS workgroups split
-// a row's key blocks further and a second launch joins their partial sums.
+// and P is rounded to bf16 for its product (2^-9 of each weight, below the output's own rounding).
 //
-// A masked pair has P = 0, which would carry a NaN or an infinity of a value to queries that do not see it: values that no
-// query of the workgroup sees are zeroed as they are loaded, and where a result is not finite its lane computes it again from
-// the keys that its query sees alone (walk_keys).
+// Up to 64 query rows a (row, kv head), bound by reading the ring: the waves of a query group split its KEYS, a wave's keys
+// and values going straight from memory to its operand registers (2 tiles a wave: 380 registers), and meet in LDS at the end,
+// weighted by their maxima; no barrier and no LDS write in the loop. 352 rows of one node over full rings, 16 q / 4 kv heads:
+// 129 us, 5.1 TB/s.
+// More query rows, bound by the products: every wave has 32 rows of its own and needs every key, so blocks pass through LDS
+// once for the four waves (128 KB: three blocks ahead, direct-to-LDS loads counted by vmcnt, one barrier a block). 128 rows of
+// 64 nodes 224 us. With 4 tiles a wave instead, from registers, the accumulators alone took half of them and the spills made
+// it 1,040 us.
+// Where few rows leave the chip short of workgroups, workgroups split a row's key blocks further and a second launch joins
+// their partial sums: a lone row of 12 nodes 12.7 + 8.6 us.
+//
+// A masked pair has P = 0, which would carry a NaN or an infinity of a value to queries that do not see it: a query row with a
+// result that is not finite is computed again from the keys that it sees alone (walk_keys).
 #include <math.h>
+#include <stddef.h>
 
 #include "hsg_common.h"
 
@@ -113,13 +120,9 @@ __device__ __forceinline__ void walk_keys(const TreeAttnParams& p, const TreeKey
   const uint16_t* q = ro.q + l * p.q_sl + (row - l * p.G) * p.q_sg;
   const uint64_t mask = mask_of(ro.masks, l);
   const int depth = depth_of(ro.masks, l);
-  const auto key = [&](int j, bool ring) -> const uint16_t* { return ring ? ro.ring_k + j * D : ro.k + j * p.nk_sl; };
-  const auto sees = [&](int j, bool ring) {
-    if (ring) return key_place(ro.ring_pos[j], ro.start) > depth - p.W;
-    return (mask >> j & 1) && depth_of(ro.masks, j) > depth - p.W;
-  };
   const auto score = [&](const uint16_t* k) {
     float s = 0.f;
+#pragma unroll 1
     for (int d = 0; d < D; d += 8) {
       float a[8], b[8];
       load8_bf16(q + d, a);
@@ -132,12 +135,16 @@ __device__ __forceinline__ void walk_keys(const TreeAttnParams& p, const TreeKey
   float m = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int e = 0; e < ND; ++e) y[e] = 0.f;
+#pragma unroll 1
   for (int pass = 0; pass < 2; ++pass)
+#pragma unroll 1
     for (int j = 0; j < p.W + ro.len; ++j) {
       const bool ring = j < p.W;
       const int at = ring ? j : j - p.W;
-      if (!sees(at, ring)) continue;
-      const float s = score(key(at, ring));
+      const bool sees = ring ? key_place(ro.ring_pos[at], ro.start) > depth - p.W
+                             : (mask >> at & 1) && depth_of(ro.masks, at) > depth - p.W;
+      if (!sees) continue;
+      const float s = score(ring ? ro.ring_k + at * D : ro.k + at * p.nk_sl);
       if (pass == 0) {
         m = fmaxf(m, s);
         continue;
@@ -145,6 +152,7 @@ __device__ __forceinline__ void walk_keys(const TreeAttnParams& p, const TreeKey
       const float w = expf(s - m);
       sum += w;
       const uint16_t* v = (ring ? ro.ring_v + at * D : ro.v + at * p.nv_sl) + d0;
+#pragma unroll
       for (int e = 0; e < ND; ++e) y[e] += w * bf2f(v[e]);
     }
 #pragma unroll
@@ -159,20 +167,22 @@ __device__ __forceinline__ bool all_finite(const float (&y)[ND]) {
   return odd == 0.f;
 }
 
-// ND normalised values of query `row`, gated and stored (dims d0 ..); not finite: computed again first
+// ND normalised values of query `row`, gated and stored (dims d0 ..)
 template <int ND>
-__device__ __forceinline__ void finish(const TreeAttnParams& p, const TreeKeys& ro, int row, int d0, float (&y)[ND]) {
-  if (!all_finite(y)) walk_keys(p, ro, row, d0, y);
+__device__ __forceinline__ void store_gated(const TreeAttnParams& p, const TreeKeys& ro, int row, int d0, float (&y)[ND]) {
   const int l = row / p.G, g = row - l * p.G;
   uint16_t* dst = ro.out + l * p.o_sl + g * p.o_sg + d0;
   if (ro.gate) {
     const uint16_t* src = ro.gate + l * p.g_sl + g * p.g_sg + d0;
+    u32x4 gw[ND / 8];
 #pragma unroll
-    for (int e = 0; e < ND; e += 8) {
+    for (int e = 0; e < ND / 8; ++e) gw[e] = load16(src + 8 * e);
+#pragma unroll
+    for (int e = 0; e < ND / 8; ++e) {
       float gt[8];
-      load8_bf16(src + e, gt);
+      unpack8(gw[e], gt);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[e + i] *= sigmoidf_(gt[i]);
+      for (int i = 0; i < 8; ++i) y[8 * e + i] *= sigmoidf_(gt[i]);
     }
   }
 #pragma unroll
@@ -184,19 +194,45 @@ __device__ __forceinline__ void finish(const TreeAttnParams& p, const TreeKeys& 
   }
 }
 
-template <int T, int KW>
-__global__ __launch_bounds__(64 * NW) void tree_attn_kernel(const TreeAttnParams p) {
+// byte offset of an LDS pointer
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+// 1 KB from memory into LDS without a register between: lane l's 16 bytes at byte `off` of `base` go to byte `to` + 16 l.
+// Counted by vmcnt in the order of issue.
+__device__ __forceinline__ void load_lds16(const void* base, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
+}
+
+struct KeyStage {
+  u32x4 k[2][D / 32][64];   // A operands of the scores, in the order of the lanes
+  uint16_t v[KB][D];        // row by row
+};
+
+template <int T, int KW, bool STAGED>
+struct TreeAttnLds {
+  static constexpr int QW = NW / KW;
+  static constexpr int STAGES = STAGED ? 4 : 1;
+  union {
+    struct {
+      u32x4 q[STAGED ? 1 : QW * T][D / 32][64];   // the queries' operands, in the order of the lanes
+    };
+    KeyStage stage[STAGES];
+    f32x4 o[KW > 1 ? NW : 1][16][64];             // a tile's partial sums of every wave
+  };
+  int kp[W_MAX + MOST];       // places of the ring's keys before the start; then the nodes' depths
+  uint32_t flags[BLOCKS];     // bit 0: some query may see a key of the block; 1: all see all
+  float ml[NW][T][16][2];
+  uint32_t odd[QW * T];       // query rows with a result that is not finite
+  __device__ TreeAttnLds() {}
+};
+
+template <int T, int KW, bool STAGED>
+__global__ __launch_bounds__(64 * NW, T == 1 ? 2 : 1) void tree_attn_kernel(const TreeAttnParams p) {
   constexpr int QW = NW / KW;
   constexpr int ROWS = 16 * T * QW;     // query rows of the workgroup
-  constexpr bool Q_LDS = T > 2;         // the queries' operands stay in LDS, in the order of the lanes, not in registers
-  __shared__ union __align__(16) Lds {
-    u32x4 q[QW * T][D / 32][64];
-    f32x4 o[NW][16][64];                // a tile's partial sums of every wave
-    __device__ Lds() {}
-  } lds;
-  __shared__ __align__(16) int kp[W_MAX + MOST];   // places of the ring's keys before the start; then the nodes' depths
-  __shared__ uint32_t flags[BLOCKS];               // bit 0: some query may see a key of the block; 1: all see all
-  __shared__ float ml[NW][T][16][2];
+  __shared__ __align__(16) TreeAttnLds<T, KW, STAGED> lds;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wk = wave % KW, wq = wave / KW;
@@ -223,7 +259,7 @@ __global__ __launch_bounds__(64 * NW) void tree_attn_kernel(const TreeAttnParams
   const int n_blocks = RB + l_hi / KB + 1;
 
   // ---- queries, and places of the keys ----
-  bf16x8 qr[Q_LDS ? 1 : T][D / 32];
+  bf16x8 qr[STAGED ? T : 1][D / 32];
   uint64_t mask[T];
   int depth[T];
 #pragma unroll
@@ -233,7 +269,7 @@ __global__ __launch_bounds__(64 * NW) void tree_attn_kernel(const TreeAttnParams
     const uint16_t* src = ro.q + l * p.q_sl + (row - l * G) * p.q_sg + 8 * g4;
     mask[t] = mask_of(ro.masks, l);
     depth[t] = depth_of(ro.masks, l);
-    if constexpr (!Q_LDS) {
+    if constexpr (STAGED) {
 #pragma unroll
       for (int ks = 0; ks < D / 32; ++ks) qr[t][ks] = as_bf16x8(load16(src + 32 * ks));
     } else {
@@ -245,17 +281,18 @@ __global__ __launch_bounds__(64 * NW) void tree_attn_kernel(const TreeAttnParams
   }
   for (int col = threadIdx.x; col < W_MAX; col += 64 * NW) {
     const int place = col < W ? key_place(ro.ring_pos[min(col, W - 1)], ro.start) : KP_NONE;
-    kp[col] = place;
+    lds.kp[col] = place;
     const uint64_t some = __ballot(place > -W), all = __ballot(place > len - 1 - W);
     if (lane == 0) {
-      flags[col / KB] = ((uint32_t)some ? 1u : 0u) | ((uint32_t)all == ~0u ? 2u : 0u);
-      flags[col / KB + 1] = ((uint32_t)(some >> 32) ? 1u : 0u) | ((uint32_t)(all >> 32) == ~0u ? 2u : 0u);
+      lds.flags[col / KB] = ((uint32_t)some ? 1u : 0u) | ((uint32_t)all == ~0u ? 2u : 0u);
+      lds.flags[col / KB + 1] = ((uint32_t)(some >> 32) ? 1u : 0u) | ((uint32_t)(all >> 32) == ~0u ? 2u : 0u);
     }
   }
   if (threadIdx.x < MOST) {
     const int i = min((int)threadIdx.x, len - 1);
-    kp[W_MAX + threadIdx.x] = depth_of(ro.masks, i);
+    lds.kp[W_MAX + threadIdx.x] = depth_of(ro.masks, i);
   }
+  if (threadIdx.x < QW * T) lds.odd[threadIdx.x] = 0u;
   __syncthreads();
 
   // ---- the wave's key blocks ----
@@ -272,101 +309,47 @@ __global__ __launch_bounds__(64 * NW) void tree_attn_kernel(const TreeAttnParams
       for (int i = 0; i < 8; ++i) O[t][hh][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
   const int step = KW * p.splits;
-  const auto next_block = [&](int b) {   // the wave's next block that a query may see
+  const auto next_block = [&](int b) {   // the next of the wave's blocks that a query may see
     for (b += step; b < n_blocks; b += step)
-      if (b >= RB || (__builtin_amdgcn_readfirstlane(flags[b]) & 1u)) break;
+      if (b >= RB || (__builtin_amdgcn_readfirstlane(lds.flags[b]) & 1u)) break;
     return b;
   };
-  u32x4 kr[2][D / 32];
-  const auto load_keys = [&](int b) __attribute__((always_inline)) {
+  // probabilities of block b for the scores S, rounded; the accumulators follow a maximum that has moved
+  const auto softmax = [&](int b, f32x4 (&S)[T][2], bf16x8 (&pb)[T]) __attribute__((always_inline)) {
     const bool ring = b < RB;
-    const uint16_t* base = ring ? ro.ring_k + b * (KB * D) : ro.k + (int64_t)(b - RB) * KB * p.nk_sl;
-    const int64_t st = ring ? D : p.nk_sl;
-    const int last = ring ? KB - 1 : len - 1 - (b - RB) * KB;
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const uint16_t* src = base + min(16 * kt + c, last) * st + 8 * g4;
-#pragma unroll
-      for (int ks = 0; ks < D / 32; ++ks) kr[kt][ks] = load16(src + 32 * ks);
-    }
-  };
-  int b = tiles > 0 ? next_block(wk + KW * split - step) : n_blocks;
-  if (b < n_blocks) load_keys(b);
-  while (b < n_blocks) {
-    const bool ring = b < RB;
-    const bool full = ring && (__builtin_amdgcn_readfirstlane(flags[b]) & 2u);
-    // ---- values: dims 128 hh + 8 c .. + 7 of keys 16 (s / 4) + 4 g4 + s % 4 ----
-    u32x4 vr[2][8];
-    {
-      const uint16_t* base = ring ? ro.ring_v + b * (KB * D) : ro.v + (int64_t)(b - RB) * KB * p.nv_sl;
-      const int64_t st = ring ? D : p.nv_sl;
-      const int last = ring ? KB - 1 : len - 1 - (b - RB) * KB;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const uint16_t* src = base + min(16 * (s >> 2) + 4 * g4 + (s & 3), last) * st + 8 * c;
-        vr[0][s] = load16(src);
-        vr[1][s] = load16(src + 128);
-      }
-    }
-    // ---- scores ----
-    f32x4 S[T][2];
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      S[t][0] = S[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      if (t >= tiles) continue;
-#pragma unroll
-      for (int ks = 0; ks < D / 32; ++ks) {
-        bf16x8 qf;
-        if constexpr (Q_LDS) qf = as_bf16x8(lds.q[wq * T + t][ks][lane]);
-        else qf = qr[t][ks];
-        S[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[0][ks]), qf, S[t][0], 0, 0, 0);
-        S[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[1][ks]), qf, S[t][1], 0, 0, 0);
-      }
-    }
-    const int b_now = b;
-    b = next_block(b);
-    if (b < n_blocks) load_keys(b);
-    // ---- masks ----
-    i32x4 place[2];
-    if (!full) {
-      const int at = (ring ? b_now * KB : W_MAX + (b_now - RB) * KB) + 4 * g4;
-      place[0] = *reinterpret_cast<const i32x4*>(&kp[at]);
-      place[1] = *reinterpret_cast<const i32x4*>(&kp[at + 16]);
-      // a value that no query of the row sees may hold anything
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const int key = 16 * (s >> 2) + 4 * g4 + (s & 3);
-        const bool live = ring ? place[s >> 2][s & 3] > -W : (b_now - RB) * KB + key <= l_hi;
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) vr[hh][s] = live ? vr[hh][s] : (u32x4){0u, 0u, 0u, 0u};
-      }
-    }
+    const bool full = ring && (__builtin_amdgcn_readfirstlane(lds.flags[b]) & 2u);
     float top[T];
     bool move = false;
+    if (full) {
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) S[t][e >> 2][e & 3] *= sl2;
+    } else {
+      const int at = (ring ? b * KB : W_MAX + (b - RB) * KB) + 4 * g4;
+      i32x4 place[2];
+      place[0] = *reinterpret_cast<const i32x4*>(&lds.kp[at]);
+      place[1] = *reinterpret_cast<const i32x4*>(&lds.kp[at + 16]);
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const uint32_t bits = ring ? ~0u : (uint32_t)(mask[t] >> ((b - RB) * KB)) >> (4 * g4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool ok = place[e >> 2][e & 3] > depth[t] - W && (bits >> (16 * (e >> 2) + (e & 3)) & 1u);
+          S[t][e >> 2][e & 3] = ok ? S[t][e >> 2][e & 3] * sl2 : -INFINITY;
+        }
+      }
+    }
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      top[t] = -INFINITY;
-      if (t >= tiles) continue;
-      const uint32_t bits = (uint32_t)(mask[t] >> (ring ? 0 : (b_now - RB) * KB)) >> (4 * g4);
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float s = S[t][kt][r] * sl2;
-          if (!full) {
-            const bool ok = place[kt][r] > depth[t] - W && (ring || (bits >> (16 * kt + r) & 1u));
-            s = ok ? s : -INFINITY;
-          }
-          S[t][kt][r] = s;
-          top[t] = fmaxf(top[t], s);
-        }
+      top[t] = fmaxf(fmaxf(fmaxf(S[t][0][0], S[t][0][1]), fmaxf(S[t][0][2], S[t][0][3])),
+                     fmaxf(fmaxf(S[t][1][0], S[t][1][1]), fmaxf(S[t][1][2], S[t][1][3])));
       top[t] = max_pair32(max_pair16(top[t]));
       move |= top[t] > m[t] + SLACK;
     }
     if (__any(move)) {
 #pragma unroll
       for (int t = 0; t < T; ++t) {
-        if (t >= tiles) continue;
         const float to = top[t] > m[t] + SLACK ? top[t] : m[t];
         const float alpha = to == -INFINITY ? 1.f : exp2_fast(m[t] - to);
         m[t] = to;
@@ -377,7 +360,6 @@ __global__ __launch_bounds__(64 * NW) void tree_attn_kernel(const TreeAttnParams
           for (int i = 0; i < 8; ++i) O[t][hh][i] *= alpha;
       }
     }
-    bf16x8 pb[T];
 #pragma unroll
     for (int t = 0; t < T; ++t) {
       const float base = m[t] == -INFINITY ? 0.f : m[t];
@@ -390,82 +372,226 @@ __global__ __launch_bounds__(64 * NW) void tree_attn_kernel(const TreeAttnParams
       }
       pb[t] = as_bf16x8(w);
     }
-    // ---- O^T += V^T . P^T ----
+  };
+  // O^T += V^T . P^T for dims 128 hh + 8 c .. + 7 of the lane's keys 16 (s / 4) + 4 g4 + s % 4
+  const auto add_values = [&](int hh, const u32x4 (&v)[8], const bf16x8 (&pb)[T]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh)
+    for (int i = 0; i < 8; ++i) {
+      u32x4 w;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        u32x4 w;
+      for (int e = 0; e < 4; ++e)
+        w[e] = __builtin_amdgcn_perm(v[2 * e + 1][i >> 1], v[2 * e][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          w[e] = __builtin_amdgcn_perm(vr[hh][2 * e + 1][i >> 1], vr[hh][2 * e][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
+      for (int t = 0; t < T; ++t)
+        O[t][hh][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(w), pb[t], O[t][hh][i], 0, 0, 0);
+    }
+  };
+
+  if constexpr (!STAGED) {
+    // keys and values straight from memory to the operand registers: a block's values are loaded before its scores, the next
+    // block's keys after them
+    u32x4 kr[2][D / 32], vr[2][8];
+    const auto load_keys = [&](int b) __attribute__((always_inline)) {
+      const bool ring = b < RB;
+      const uint16_t* base = ring ? ro.ring_k + b * (KB * D) : ro.k + (int64_t)(b - RB) * KB * p.nk_sl;
+      const uint32_t st = ring ? D : (uint32_t)p.nk_sl;
+      const int last = ring ? KB - 1 : len - 1 - (b - RB) * KB;
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-          if (t >= tiles) continue;
-          O[t][hh][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(w), pb[t], O[t][hh][i], 0, 0, 0);
+      for (int kt = 0; kt < 2; ++kt) {
+        const uint32_t off = (uint32_t)min(16 * kt + c, last) * st + 8 * g4;
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ++ks) kr[kt][ks] = load16(base + off + 32 * ks);
+      }
+    };
+    int b = tiles > 0 ? next_block(wk + KW * split - step) : n_blocks;
+    if (b < n_blocks) load_keys(b);
+    while (b < n_blocks) {
+      const bool ring = b < RB;
+      {
+        const uint16_t* base = ring ? ro.ring_v + b * (KB * D) : ro.v + (int64_t)(b - RB) * KB * p.nv_sl;
+        const uint32_t st = ring ? D : (uint32_t)p.nv_sl;
+        const int last = ring ? KB - 1 : len - 1 - (b - RB) * KB;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          const uint32_t off = (uint32_t)min(16 * (s >> 2) + 4 * g4 + (s & 3), last) * st + 8 * c;
+          vr[0][s] = load16(base + off);
+          vr[1][s] = load16(base + off + 128);
         }
       }
-  }
-
-  // ---- the waves' partial sums meet ----
+      f32x4 S[T][2];
 #pragma unroll
-  for (int t = 0; t < T; ++t) {
-    sum[t] = add_xor32(add_xor16(sum[t]));
-    if (g4 == 0) {
-      ml[wave][t][c][0] = m[t];
-      ml[wave][t][c][1] = sum[t];
+      for (int t = 0; t < T; ++t) S[t][0] = S[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ++ks)
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          const bf16x8 qf = as_bf16x8(lds.q[wq * T + t][ks][lane]);
+          S[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[0][ks]), qf, S[t][0], 0, 0, 0);
+          S[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[1][ks]), qf, S[t][1], 0, 0, 0);
+        }
+      const int b_now = b;
+      b = next_block(b);
+      if (b < n_blocks) load_keys(b);
+      bf16x8 pb[T];
+      softmax(b_now, S, pb);
+      add_values(0, vr[0], pb);
+      add_values(1, vr[1], pb);
+    }
+  } else {
+    // every wave needs every block: blocks pass through LDS, three ahead of the one at work
+    constexpr int AHEAD = TreeAttnLds<T, KW, STAGED>::STAGES - 1;
+    constexpr int EACH = 2 * KB * D * 2 / 1024 / NW;      // a wave's loads of a block
+    const auto fetch = [&](int b, int stage) __attribute__((always_inline)) {
+      const bool ring = b < RB;
+      const uint16_t* kb = ring ? ro.ring_k + b * (KB * D) : ro.k + (int64_t)(b - RB) * KB * p.nk_sl;
+      const uint16_t* vb = ring ? ro.ring_v + b * (KB * D) : ro.v + (int64_t)(b - RB) * KB * p.nv_sl;
+      const uint32_t k_st = ring ? D : (uint32_t)p.nk_sl, v_st = ring ? D : (uint32_t)p.nv_sl;
+      const int last = ring ? KB - 1 : len - 1 - (b - RB) * KB;
+      const uint32_t to = lds_offset(&lds.stage[stage]);
+#pragma unroll
+      for (int e = 0; e < EACH / 2; ++e) {
+        const int o = wave * (EACH / 2) + e;              // (key tile, k step) of the keys; two rows of the values
+        const uint32_t k_off = (uint32_t)min(16 * (o >> 3) + c, last) * k_st + 32 * (o & 7) + 8 * g4;
+        load_lds16(kb, 2 * k_off, __builtin_amdgcn_readfirstlane(to + 1024 * o));
+        const uint32_t v_off = (uint32_t)min(2 * o + (lane >> 5), last) * v_st + 8 * (lane & 31);
+        load_lds16(vb, 2 * v_off, __builtin_amdgcn_readfirstlane(to + (uint32_t)offsetof(KeyStage, v) + 1024 * o));
+      }
+    };
+    int ahead = next_block(split - step);                 // the next block to fetch
+    int b = ahead;
+    int stage = 0, fetched = 0;                           // blocks fetched and not yet worked on, after b
+    for (; fetched < AHEAD && ahead < n_blocks; ++fetched) {
+      fetch(ahead, fetched);
+      ahead = next_block(ahead);
+    }
+    while (b < n_blocks) {
+      // the oldest block has landed: at most the later ones' loads are outstanding
+      if (fetched >= 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * EACH) : "memory");
+      else if (fetched == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(EACH) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();                       // for every wave; and the block before is read no more
+      asm volatile("" ::: "memory");
+      --fetched;
+      if (ahead < n_blocks) {
+        fetch(ahead, (stage + AHEAD) % (AHEAD + 1));
+        ahead = next_block(ahead);
+        ++fetched;
+      }
+      if (tiles > 0) {
+        const KeyStage& ks_ = lds.stage[stage];
+        f32x4 S[T][2];
+#pragma unroll
+        for (int t = 0; t < T; ++t) S[t][0] = S[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ++ks) {
+          const bf16x8 k0 = as_bf16x8(ks_.k[0][ks][lane]), k1 = as_bf16x8(ks_.k[1][ks][lane]);
+#pragma unroll
+          for (int t = 0; t < T; ++t) {
+            S[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qr[t][ks], S[t][0], 0, 0, 0);
+            S[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qr[t][ks], S[t][1], 0, 0, 0);
+          }
+        }
+        bf16x8 pb[T];
+        softmax(b, S, pb);
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          u32x4 vr[8];
+#pragma unroll
+          for (int s = 0; s < 8; ++s)
+            vr[s] = *reinterpret_cast<const u32x4*>(&ks_.v[16 * (s >> 2) + 4 * g4 + (s & 3)][128 * hh + 8 * c]);
+          add_values(hh, vr, pb);
+        }
+      }
+      b = next_block(b);
+      stage = (stage + 1) % (AHEAD + 1);
     }
   }
-  __syncthreads();   // (the queries in LDS are read no more, either)
+
+  // ---- the waves' partial sums meet; outputs ----
+#pragma unroll
+  for (int t = 0; t < T; ++t) sum[t] = add_xor32(add_xor16(sum[t]));
+  if constexpr (KW > 1) {
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+      if (g4 == 0) {
+        lds.ml[wave][t][c][0] = m[t];
+        lds.ml[wave][t][c][1] = sum[t];
+      }
+    __syncthreads();   // (the queries in LDS are read no more, either)
+  }
+  // lane (g4, c) of product (hh, i), register r: query c, dim 128 hh + 32 g4 + 8 r + i; a lane stores 8 R dims at a time
+  constexpr int R = KW > 1 ? 8 / KW : 4;
+  constexpr int TIMES = KW > 1 ? 1 : 2;
 #pragma unroll
   for (int t = 0; t < T; ++t) {
-    float top = -INFINITY, total = 0.f;
-#pragma unroll
-    for (int w = 0; w < KW; ++w) top = fmaxf(top, ml[wq * KW + w][t][c][0]);
-    const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int w = 0; w < KW; ++w) total += exp2_fast(ml[wq * KW + w][t][c][0] - base) * ml[wq * KW + w][t][c][1];
-    const float mine = exp2_fast(m[t] - base);
-    if (t) __syncthreads();   // the tile before is read
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) lds.o[wave][8 * hh + i][lane] = O[t][hh][i] * mine;
-    __syncthreads();
-    // lane (g4, c) of product (hh, i), register r: query c, dim 128 hh + 32 g4 + 8 r + i
-    constexpr int R = 8 / KW;           // registers of the lane: with KW waves 1 of KW pieces of the 2 x 4
-    const int hh = wk * R / 4, r0 = wk * R % 4;
-    float y[8 * R];
-#pragma unroll
-    for (int e = 0; e < 8 * R; ++e) y[e] = 0.f;
-#pragma unroll
-    for (int w = 0; w < KW; ++w)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float* src = reinterpret_cast<const float*>(&lds.o[wq * KW + w][8 * hh + i][lane]) + r0;
-#pragma unroll
-        for (int r = 0; r < R; ++r) y[8 * r + i] += src[r];
-      }
     const int row = r_lo + 16 * t + c;
-    const int d0 = 128 * hh + 32 * g4 + 8 * r0;
-    if (row < M) {
+    float top = m[t], total = sum[t];
+    if constexpr (KW > 1) {
+      top = -INFINITY;
+      total = 0.f;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) top = fmaxf(top, lds.ml[wq * KW + w][t][c][0]);
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) total += exp2_fast(lds.ml[wq * KW + w][t][c][0] - base) * lds.ml[wq * KW + w][t][c][1];
+      const float mine = exp2_fast(m[t] - base);
+      if (t) __syncthreads();   // the tile before is read
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) lds.o[wave][8 * hh + i][lane] = O[t][hh][i] * mine;
+      __syncthreads();
+    }
+#pragma unroll
+    for (int x = 0; x < TIMES; ++x) {
+      const int hh = KW > 1 ? wk * R / 4 : x, r0 = KW > 1 ? wk * R % 4 : 0;
+      float y[8 * R];
+      if constexpr (KW > 1) {
+#pragma unroll
+        for (int e = 0; e < 8 * R; ++e) y[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float* src = reinterpret_cast<const float*>(&lds.o[wq * KW + w][8 * hh + i][lane]) + r0;
+#pragma unroll
+            for (int r = 0; r < R; ++r) y[8 * r + i] += src[r];
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y[8 * r + i] = O[t][x][i][r];
+      }
+      const int d0 = 128 * hh + 32 * g4 + 8 * r0;
+      if (row >= M) continue;
       if (p.splits == 1) {
         const float inv = 1.0f / total;
 #pragma unroll
         for (int e = 0; e < 8 * R; ++e) y[e] *= inv;
-        finish(p, ro, row, d0, y);
+        if (!all_finite(y)) atomicOr(&lds.odd[wq * T + t], 1u << c);
+        store_gated(p, ro, row, d0, y);
       } else {
         const int64_t at = ((int64_t)pair * p.splits + split) * ((int64_t)G * p.max_nodes) + row;
         float* dst = p.part_o + at * D + d0;
 #pragma unroll
         for (int e = 0; e < 8 * R; e += 4) *reinterpret_cast<f32x4*>(dst + e) = (f32x4){y[e], y[e + 1], y[e + 2], y[e + 3]};
-        if (wk == 0 && g4 == 0) {
+        if (hh == 0 && g4 == 0 && r0 == 0) {
           p.part_ml[2 * at] = top;
           p.part_ml[2 * at + 1] = total;
         }
       }
     }
   }
+  if (p.splits > 1) return;
+  // ---- query rows with a result that is not finite: again, over the keys that they see alone ----
+  __syncthreads();   // also: the stores of these rows' first results are done
+  for (int i = threadIdx.x >> 5; i < ROWS; i += 64 * NW / 32)
+    if (lds.odd[i >> 4] >> (i & 15) & 1u) {
+      float y[8];
+      walk_keys(p, ro, r_wg + i, 8 * (threadIdx.x & 31), y);
+      store_gated(p, ro, r_wg + i, 8 * (threadIdx.x & 31), y);
+    }
 }
 
 // Joins the splits' partial sums: 16 lanes a query row, 16 dims a lane
@@ -498,7 +624,8 @@ __global__ __launch_bounds__(256) void tree_attn_join_kernel(const TreeAttnParam
   const float inv = 1.0f / total;
 #pragma unroll
   for (int e = 0; e < 16; ++e) y[e] *= inv;
-  finish(p, ro, row, d0, y);
+  if (!all_finite(y)) walk_keys(p, ro, row, d0, y);
+  store_gated(p, ro, row, d0, y);
 }
 
 // The committed chain's keys and values into the ring (of a chain longer than the window its last W), 16 nodes a workgroup:
@@ -531,15 +658,14 @@ __global__ __launch_bounds__(256) void tree_ring_write_kernel(const TreeAttnPara
   }
 }
 
-// Query rows of a workgroup, and the ways its keys are split over its waves. From 65 query rows on two waves share a query
-// group, which halves what meets in LDS at the end.
+// Query rows of a workgroup: from 65 on every wave has its own and the keys pass through LDS
 inline int rows_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 // Workgroups of a row's key blocks: few rows leave the chip (256 CUs) short of workgroups, and one CU moves only a few tens
-// of GB/s. 4 at most: then a wave has one ring block of a full window.
+// of GB/s. 8 at most.
 inline int splits_of(int64_t n_rows, int64_t hkv, int64_t rows) {
   const int64_t units = n_rows * hkv * ((rows + rows_of(rows) - 1) / rows_of(rows));
-  return units <= 64 ? 4 : units <= 128 ? 2 : 1;
+  return units <= 32 ? 8 : units <= 64 ? 4 : units <= 128 ? 2 : 1;
 }
 
 inline size_t part_bytes(int64_t n_rows, int64_t hkv, int64_t rows, int splits) {
@@ -572,6 +698,8 @@ extern "C" int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int
   if (n_rows == 0) return HSG_OK;
   if (!q || !ring_k || !ring_v || !new_k || !new_v || !ring_pos || !slots || !starts || !lens || !offsets || !masks || !out)
     return HSG_ERR_ARG;
+  // a row's keys are addressed by 32-bit byte offsets
+  if (nk_sl < 0 || nv_sl < 0 || nk_sl >= (1 << 24) || nv_sl >= (1 << 24)) return HSG_ERR_SHAPE;
   const int64_t strides[] = {q_sl, q_sh, q_sg, nk_sl, nk_sh, nv_sl, nv_sh, o_sl, o_sh, o_sg};
   for (int64_t st : strides)
     if (st % 8) return HSG_ERR_ALIGN;
@@ -604,10 +732,10 @@ extern "C" int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int
   if (blocks >= (1 << 24)) return HSG_ERR_SHAPE;   // a launch holds less than 2^32 threads
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NW), 0, st, p); };
-  if (per_wg == 16) launch(tree_attn_kernel<1, 4>);
-  else if (per_wg == 32) launch(tree_attn_kernel<2, 4>);
-  else if (per_wg == 64) launch(tree_attn_kernel<4, 4>);
-  else launch(tree_attn_kernel<4, 2>);
+  if (per_wg == 16) launch(tree_attn_kernel<1, 4, false>);
+  else if (per_wg == 32) launch(tree_attn_kernel<2, 4, false>);
+  else if (per_wg == 64) launch(tree_attn_kernel<2, 2, false>);
+  else launch(tree_attn_kernel<2, 1, true>);
   if (p.splits > 1)
     hipLaunchKernelGGL(tree_attn_join_kernel, dim3((unsigned)pairs, (unsigned)((rows + 15) / 16)), dim3(256), 0, st, p);
   if (commits)
