@@ -60,14 +60,20 @@ struct TreeStepLds {
     };
     float U[N][KD];        // walk_row
   };
-  float T[NT][16][20];     // (I + A_bb)^-1 of the diagonal blocks
+  uint16_t k[N * KD], q[N * KD];   // row by row, 16-byte pieces at kq_at
+  float T[NT][16][20];             // (I + A_bb)^-1 of the diagonal blocks
   double G[N];
-  uint64_t mask[N];        // ancestors and itself, within the row
-  float g[N], beta[N], kinv[N], qinv[N];
+  uint64_t mask[N];                // ancestors and itself, within the row
+  float g[N], beta[N], eG[N], kinv[N], qinv[N];
+  float left[N];                   // e^(G_c - G_i) on the committed chain, else 0
   float part[N][NW];
-  int odd[NW];             // a wave saw a value that is not finite
+  int odd[NW];                     // a wave saw a value that is not finite
   __device__ TreeStepLds() {}
 };
+
+// Element offset of 16-byte piece pc of row i: the pieces of a row are permuted by its number, so that reads of one piece of
+// 16 rows, and transpose reads of 4, spread over the banks
+__device__ __forceinline__ int kq_at(int i, int pc) { return i * KD + 8 * (pc ^ (i & 15)); }
 
 // One (row, value head)
 struct TreeRow {
@@ -79,6 +85,13 @@ struct TreeRow {
 
 __device__ __forceinline__ bf16x8 load_bf16x8(const uint16_t* p) {
   return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(p));
+}
+
+// LDS transpose read: within each group of 16 lanes, lane 4 q + e receives element e of the 4-value vectors that lanes q, q + 4,
+// q + 8 and q + 12 of its group address
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+__device__ __forceinline__ u32x2 ld_tr4(const uint16_t* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p)));
 }
 
 // the upper halves of two fp32 words as a bf16 pair (a in the low half)
@@ -192,7 +205,7 @@ __device__ __forceinline__ void walk_row(const TreeStepParams& p, const TreeRow&
 }
 
 template <int NT, bool HALF, bool GATED>
-__global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(const TreeStepParams p) {
+__global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(const TreeStepParams p) {
   constexpr int PARTS = HALF ? 2 : 3;
   __shared__ TreeStepLds<NT> lds;
   const int lane = threadIdx.x & 63;
@@ -216,98 +229,137 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(const TreeStepParams 
   ro.done = (int)(done64 < 0 ? 0 : done64 > len ? len : done64);
   const int col = 32 * wave + 2 * c;   // the lane's columns col, col + 1
 
+  // Loads are waited for in the order of their issue: what the first phases need is loaded before S0, what the last ones need
+  // after it.
+  // ---- k and q of a tile: NT == 4: wave = tile; else the waves from 2 on take q ----
+  constexpr bool BOTH = NT == 4;
+  const int kt = BOTH ? wave : wave % NT;
+  const bool do_k = BOTH || wave < NT, do_q = BOTH || (wave >= 2 && wave < 2 + NT);
+  const int64_t kq_row = (int64_t)min(16 * kt + c, len - 1) * p.qkv_stride + 8 * g4;
+  u32x4 kp[4], qp[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    if (do_k) kp[s] = *reinterpret_cast<const u32x4*>(ro.k + kq_row + 32 * s);
+    if (do_q) qp[s] = *reinterpret_cast<const u32x4*>(ro.q + kq_row + 32 * s);
+  }
+  const int64_t node = off + min(lane, len - 1);
+  uint64_t mask = 0;
+  float a = 0.f, b = 0.f, a_log = 0.f, dt = 0.f;
+  if (wave == 0) {
+    mask = (uint64_t)p.masks[node];
+    a = bf2f(p.a[node * p.ab_stride + hv]);
+    b = bf2f(p.b[node * p.ab_stride + hv]);
+    a_log = bf2f(p.A_log[hv]);
+    dt = bf2f(p.dt_bias[hv]);
+  }
   // ---- S0: rows 32 s + 8 g4 + i ----
-  float s0[4][2][8];
+  typedef std::conditional_t<HALF, uint32_t, f32x2> StatePair;
+  StatePair raw[4][8];
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int64_t at = ro.state_at + (32 * s + 8 * g4 + i) * KD + col;
-      if constexpr (HALF) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.state) + at);
-        s0[s][0][i] = h2f((uint16_t)w);
-        s0[s][1][i] = h2f((uint16_t)(w >> 16));
-      } else {
-        const f32x2 w = *reinterpret_cast<const f32x2*>(static_cast<const float*>(p.state) + at);
-        s0[s][0][i] = w[0];
-        s0[s][1][i] = w[1];
-      }
+      raw[s][i] = *reinterpret_cast<const StatePair*>(reinterpret_cast<const std::conditional_t<HALF, uint16_t, float>*>(p.state) + at);
     }
+  const auto s0 = [&](int s, int j, int i) {
+    if constexpr (HALF) return h2f((uint16_t)(raw[s][i] >> (16 * j)));
+    else return raw[s][i][j];
+  };
+  // ---- v and z ----
+  uint32_t vw[NT][4], zw[GATED ? NT : 1][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = min(16 * t + 4 * g4 + r, len - 1);
+      vw[t][r] = *reinterpret_cast<const uint32_t*>(ro.v + (int64_t)i * p.qkv_stride + col);
+    }
+  if constexpr (GATED) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = min(16 * t + 4 * g4 + r, len - 1);
+        zw[t][r] = *reinterpret_cast<const uint32_t*>(ro.z + (int64_t)i * p.z_stride + col);
+      }
+  }
+  __builtin_amdgcn_sched_barrier(0);   // the loads stay where they stand
 
+  // ---- k and q to LDS, and their lengths ----
+  const auto stage = [&](const u32x4 (&x)[4], uint16_t* to) {
+    float ss = 0.f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      float y[8];
+      unpack8(x[s], y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(y[i], y[i], ss);
+      *reinterpret_cast<u32x4*>(to + kq_at(16 * kt + c, 4 * s + g4)) = x[s];
+    }
+    return add_xor32(add_xor16(ss));
+  };
+  if (do_k) {
+    const float ss = stage(kp, lds.k);
+    if (g4 == 0) lds.kinv[16 * kt + c] = 1.0f / sqrtf(ss + 1e-6f);
+  }
+  if (do_q) {
+    const float ss = stage(qp, lds.q);
+    if (g4 == 0) lds.qinv[16 * kt + c] = p.scale / sqrtf(ss + 1e-6f);
+  }
   // ---- a node's scalars: lane = node ----
   if (wave == 0) {
-    const int i = min(lane, len - 1);
     const bool valid = lane < len;
     const uint64_t self = 1ull << lane;
-    uint64_t mask = (uint64_t)p.masks[off + i];
     mask = valid ? (mask & (self - 1)) | self : self;
-    const float a = bf2f(p.a[(off + i) * p.ab_stride + hv]), b = bf2f(p.b[(off + i) * p.ab_stride + hv]);
-    const float g = valid ? log_decay(a, bf2f(p.A_log[hv]), bf2f(p.dt_bias[hv])) : 0.f;
+    const float g = valid ? log_decay(a, a_log, dt) : 0.f;
     // the sum down the path, by pointer doubling
     double sum = g;
     const uint64_t above = mask & ~self;
     int up = above ? 63 - __clzll((long long)above) : -1;
-#pragma unroll
-    for (int s = 0; s < 6; ++s) {
+    for (int far = 1; far < len; far <<= 1) {
       const int at = up < 0 ? lane : up;
       const double more = __shfl(sum, at, 64);
       const int next = __shfl(up, at, 64);
       sum += up < 0 ? 0.0 : more;
       up = up < 0 ? -1 : next;
     }
+    const double Gc = __shfl(sum, max(ro.done - 1, 0), 64);
     if (lane < 16 * NT) {
       lds.mask[lane] = mask;
       lds.g[lane] = g;
       lds.G[lane] = sum;
+      lds.eG[lane] = expf((float)sum);
+      lds.left[lane] = lane < ro.done ? expf((float)(Gc - sum)) : 0.f;
       lds.beta[lane] = valid ? sigmoid_f32(b) : 0.f;
-    }
-  }
-  // ---- the lengths of k and q: wave = tile ----
-  const auto row_of = [&](int t) { return (int64_t)min(16 * t + c, len - 1) * p.qkv_stride; };   // an operand's row
-  if (wave < NT) {
-    float kk = 0.f, qq = 0.f;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      float x[8];
-      load8_bf16(ro.k + row_of(wave) + 32 * s + 8 * g4, x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) kk = __builtin_fmaf(x[i], x[i], kk);
-      load8_bf16(ro.q + row_of(wave) + 32 * s + 8 * g4, x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) qq = __builtin_fmaf(x[i], x[i], qq);
-    }
-    kk = add_xor32(add_xor16(kk));
-    qq = add_xor32(add_xor16(qq));
-    if (g4 == 0) {
-      lds.kinv[16 * wave + c] = 1.0f / sqrtf(kk + 1e-6f);
-      lds.qinv[16 * wave + c] = p.scale / sqrtf(qq + 1e-6f);
     }
   }
   lds_barrier();
 
-  // ---- -A and P: (block pair, which of the two) dealt over the waves ----
-  for (int it = wave; it < NT * (NT + 1); it += NW) {
-    const int pair = it >> 1;
-    const bool is_q = it & 1;
+  const auto k_part = [&](int t, int s) { return load_bf16x8(&lds.k[kq_at(16 * t + c, 4 * s + g4)]); };
+  const auto q_part = [&](int t, int s) { return load_bf16x8(&lds.q[kq_at(16 * t + c, 4 * s + g4)]); };
+  // ---- -A and P, block pairs dealt over the waves ----
+  for (int pair = wave; pair < NT * (NT + 1) / 2; pair += NW) {
     const int bi = pair < 1 ? 0 : pair < 3 ? 1 : pair < 6 ? 2 : 3;
     const int bj = pair - bi * (bi + 1) / 2;
     if (bi >= tiles) break;
-    const uint16_t* x = (is_q ? ro.q : ro.k) + row_of(bi) + 8 * g4;
-    const uint16_t* y = ro.k + row_of(bj) + 8 * g4;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(load_bf16x8(x + 32 * s), load_bf16x8(y + 32 * s), acc, 0, 0, 0);
+    for (int s = 0; s < 4; ++s) {
+      const bf16x8 y = k_part(bj, s);
+      kk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k_part(bi, s), y, kk, 0, 0, 0);
+      qk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q_part(bi, s), y, qk, 0, 0, 0);
+    }
     const int j = 16 * bj + c;
     const double Gj = lds.G[j];
     const float kj = lds.kinv[j];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * bi + 4 * g4 + r;
-      const bool on = (lds.mask[i] >> j & 1) && i < len && (is_q || i != j);
-      const float d = expf((float)(lds.G[i] - Gj)) * kj * acc[r];
-      if (is_q) lds.P[i][j] = on ? lds.qinv[i] * d : 0.f;
-      else lds.A[i][j] = on ? -lds.beta[i] * lds.kinv[i] * d : 0.f;
+      const bool on = (lds.mask[i] >> j & 1) && i < len;
+      const float d = expf((float)(lds.G[i] - Gj)) * kj;
+      lds.P[i][j] = on ? lds.qinv[i] * d * qk[r] : 0.f;
+      lds.A[i][j] = on && i != j ? -lds.beta[i] * lds.kinv[i] * d * kk[r] : 0.f;
     }
   }
   lds_barrier();
@@ -316,11 +368,13 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(const TreeStepParams 
   if (wave < tiles) {
     float t[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float acc = i == c ? 1.f : 0.f;
+    for (int i = 0; i < 16; ++i) t[i] = i == c ? 1.f : 0.f;
+    const int rows = min(16, len - 16 * wave);
 #pragma unroll
-      for (int m = 0; m < i; ++m) acc = __builtin_fmaf(lds.A[16 * wave + i][16 * wave + m], t[m], acc);
-      t[i] = acc;
+    for (int m = 0; m < 15; ++m) {   // t[m] is settled: its share of the rows below
+      if (m + 1 >= rows) break;
+#pragma unroll
+      for (int i = m + 1; i < 16; ++i) t[i] = __builtin_fmaf(lds.A[16 * wave + i][16 * wave + m], t[m], t[i]);
     }
     if (g4 == 0) {
 #pragma unroll
@@ -338,16 +392,20 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(const TreeStepParams 
   for (int s = 0; s < 4; ++s) {
     bf16x8 part[2][PARTS];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) split8<PARTS>(s0[s][j], part[j]);
+    for (int j = 0; j < 2; ++j) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = s0(s, j, i);
+      split8<PARTS>(x, part[j]);
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if (t >= tiles) break;
-      const bf16x8 kf = load_bf16x8(ro.k + row_of(t) + 32 * s + 8 * g4);
-      const bf16x8 qf = load_bf16x8(ro.q + row_of(t) + 32 * s + 8 * g4);
+      const bf16x8 kf = k_part(t, s), qf = q_part(t, s);
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int w = PARTS - 1; w >= 0; --w)
 #pragma unroll
-        for (int w = PARTS - 1; w >= 0; --w) {
+        for (int j = 0; j < 2; ++j) {
           u[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, part[j][w], u[t][j], 0, 0, 0);
           o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf, part[j][w], o[t][j], 0, 0, 0);
         }
@@ -357,17 +415,17 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(const TreeStepParams 
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (t >= tiles) break;
+    const int i0 = 16 * t + 4 * g4;
+    const f32x4 e = *reinterpret_cast<const f32x4*>(&lds.eG[i0]), be = *reinterpret_cast<const f32x4*>(&lds.beta[i0]);
+    const f32x4 ki = *reinterpret_cast<const f32x4*>(&lds.kinv[i0]), qi = *reinterpret_cast<const f32x4*>(&lds.qinv[i0]);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * t + 4 * g4 + r;
-      const uint32_t vw = *reinterpret_cast<const uint32_t*>(ro.v + (int64_t)min(i, len - 1) * p.qkv_stride + col);
       float v[2];
-      unpack2(vw, v[0], v[1]);
-      const float e = expf((float)lds.G[i]);
+      unpack2(vw[t][r], v[0], v[1]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        u[t][j][r] = i < len ? lds.beta[i] * (v[j] - e * lds.kinv[i] * u[t][j][r]) : 0.f;
-        o[t][j][r] *= e * lds.qinv[i];
+        u[t][j][r] = i0 + r < len ? be[r] * (v[j] - e[r] * ki[r] * u[t][j][r]) : 0.f;
+        o[t][j][r] *= e[r] * qi[r];
       }
     }
   }
@@ -441,7 +499,7 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(const TreeStepParams 
         const f32x4 ss = *reinterpret_cast<const f32x4*>(lds.part[i]);
         const float rs = rsqrtf(((ss[0] + ss[1]) + (ss[2] + ss[3])) * (1.0f / KD) + p.eps);
         float z[2];
-        unpack2(*reinterpret_cast<const uint32_t*>(ro.z + (int64_t)min(i, len - 1) * p.z_stride + col), z[0], z[1]);
+        unpack2(zw[t][r], z[0], z[1]);
 #pragma unroll
         for (int j = 0; j < 2; ++j) y[j] *= rs * nw[j] * siluf_(z[j]);
       }
@@ -449,39 +507,55 @@ __global__ __launch_bounds__(64 * NW) void gdn_tree_kernel(const TreeStepParams 
     }
   }
 
-  // ---- the committed chain moves the state ----
+  // ---- the committed chain moves the state: u scaled, split as the state was, times k^T read from LDS transposed ----
   if (ro.done > 0) {
-    const double Gc = lds.G[ro.done - 1];
-    const float ec = expf((float)Gc);
+    const float ec = lds.eG[ro.done - 1];
+    constexpr int NP = (NT + 1) / 2;     // pairs of tiles: a product takes 32 nodes, the lane's own 4 of either tile
+    bf16x8 up[NP][2][3];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t2 = 0; t2 < NP; ++t2) {
+      float x[2][8] = {};
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * t + 4 * g4 + r;
-        const float d = i < ro.done ? expf((float)(Gc - lds.G[i])) * lds.kinv[i] : 0.f;
+      for (int hh = 0; hh < 2; ++hh) {
+        const int t = 2 * t2 + hh;
+        if (t >= NT) break;
+        const int i0 = 16 * t + 4 * g4;
+        const f32x4 le = *reinterpret_cast<const f32x4*>(&lds.left[i0]), ki = *reinterpret_cast<const f32x4*>(&lds.kinv[i0]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) u[t][j][r] *= d;
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) x[j][4 * hh + r] = i0 + r < ro.done ? u[t][j][r] * (le[r] * ki[r]) : 0.f;
       }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) split8<3>(x[j], up[t2][j]);
+    }
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
-        // accumulator row 4 g4 + r is state row 32 s + 8 g4 + 4 hh + r
+        // accumulator row 4 g4 + r is state row 32 s + 8 g4 + 4 hh + r: operand row m = c is k's dim 32 s + 8 (c / 4) + 4 hh
+        // + c % 4, which transpose reads of 4-value vectors 8 dims apart give
         f32x4 acc[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[j][r] = ec * s0[s][j][4 * hh + r];
-        const uint16_t* kcol = ro.k + 32 * s + 8 * (c >> 2) + 4 * hh + (c & 3);
+          for (int r = 0; r < 4; ++r) acc[j][r] = ec * s0(s, j, 4 * hh + r);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if (16 * t >= ro.done) break;
+        for (int t2 = 0; t2 < NP; ++t2) {
+          if (32 * t2 >= ro.done) break;
+          const auto four = [&](int t) {
+            const int i = 16 * t + 4 * g4 + (c >> 2);   // this lane's address: node row, vector c % 4
+            return ld_tr4(&lds.k[kq_at(i, 4 * s + (c & 3)) + 4 * hh]);
+          };
+          const u32x2 lo = four(2 * t2);
+          u32x2 hi = {0u, 0u};
+          if (2 * t2 + 1 < NT) hi = four(min(2 * t2 + 1, NT - 1));
+          const bf16x8 kf = __builtin_bit_cast(bf16x8, (u32x4){lo[0], lo[1], hi[0], hi[1]});
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float kv = bf2f(kcol[(int64_t)min(16 * t + 4 * g4 + r, ro.done - 1) * p.qkv_stride]);
+          for (int w = 2; w >= 0; --w)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv, u[t][j][r], acc[j], 0, 0, 0);
-          }
+            for (int j = 0; j < 2; ++j)
+              acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, up[t2][j][w], acc[j], 0, 0, 0);
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
