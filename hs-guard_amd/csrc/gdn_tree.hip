@@ -61,7 +61,7 @@ struct TreeStepLds {
     float U[N][KD];        // walk_row
   };
   uint16_t k[N * KD], q[N * KD];   // row by row, 16-byte pieces at kq_at
-  float T[NT][16][20];             // (I + A_bb)^-1 of the diagonal blocks
+  f32x4 T[NT][64];                 // (I + A_bb)^-1 of the diagonal blocks, as the A operand of a lane
   double G[N];
   uint64_t mask[N];                // ancestors and itself, within the row
   float g[N], beta[N], eG[N], kinv[N], qinv[N];
@@ -204,8 +204,9 @@ __device__ __forceinline__ void walk_row(const TreeStepParams& p, const TreeRow&
   }
 }
 
-template <int NT, bool HALF, bool GATED>
-__global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(const TreeStepParams p) {
+// MOVES: rows may commit. Without, S0's registers are free as soon as it is split, and small trees keep three workgroups on a CU.
+template <int NT, bool HALF, bool GATED, bool MOVES>
+__global__ __launch_bounds__(64 * NW, NT == 1 && !MOVES ? 3 : 2) void gdn_tree_kernel(const TreeStepParams p) {
   constexpr int PARTS = HALF ? 2 : 3;
   __shared__ TreeStepLds<NT> lds;
   const int lane = threadIdx.x & 63;
@@ -213,7 +214,7 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(cons
   const int g4 = lane >> 4, c = lane & 15;
   const int n = blockIdx.x / p.HV, hv = blockIdx.x - n * p.HV;
   const int64_t slot = p.slots[n], len64 = p.lens[n], off = p.offsets[n];
-  const int64_t done64 = p.commits ? p.commits[n] : 0;
+  const int64_t done64 = MOVES ? p.commits[n] : 0;
   if ((slot < 0) | (slot >= p.state_rows) | (len64 <= 0) | (len64 > p.max_nodes)) return;
   const int len = (int)len64;
   const int tiles = (len + 15) >> 4;
@@ -231,16 +232,21 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(cons
 
   // Loads are waited for in the order of their issue: what the first phases need is loaded before S0, what the last ones need
   // after it.
-  // ---- k and q of a tile: NT == 4: wave = tile; else the waves from 2 on take q ----
+  // ---- k and q of a tile: with 4 tiles wave = tile; else waves from 0 on take k, waves from 2 on q ----
   constexpr bool BOTH = NT == 4;
   const int kt = BOTH ? wave : wave % NT;
-  const bool do_k = BOTH || wave < NT, do_q = BOTH || (wave >= 2 && wave < 2 + NT);
-  const int64_t kq_row = (int64_t)min(16 * kt + c, len - 1) * p.qkv_stride + 8 * g4;
-  u32x4 kp[4], qp[4];
+  const bool is_q = !BOTH && wave >= 2, idle = !BOTH && (wave & 1) >= NT;
+  // (lane offsets are 32 bits on a uniform base: 64-bit addresses per lane cost the registers that a third workgroup needs)
+  const uint32_t stride = (uint32_t)p.qkv_stride;
+  const uint32_t kq_row = (uint32_t)min(16 * kt + c, len - 1) * stride + 8 * g4;
+  u32x4 kp[4], qp[BOTH ? 4 : 1];
+  if (!idle) {
+    const uint16_t* const src = is_q ? ro.q : ro.k;
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    if (do_k) kp[s] = *reinterpret_cast<const u32x4*>(ro.k + kq_row + 32 * s);
-    if (do_q) qp[s] = *reinterpret_cast<const u32x4*>(ro.q + kq_row + 32 * s);
+    for (int s = 0; s < 4; ++s) {
+      kp[s] = *reinterpret_cast<const u32x4*>(src + 32 * s + kq_row);
+      if constexpr (BOTH) qp[s] = *reinterpret_cast<const u32x4*>(ro.q + 32 * s + kq_row);
+    }
   }
   const int64_t node = off + min(lane, len - 1);
   uint64_t mask = 0;
@@ -254,14 +260,14 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(cons
   }
   // ---- S0: rows 32 s + 8 g4 + i ----
   typedef std::conditional_t<HALF, uint32_t, f32x2> StatePair;
+  typedef std::conditional_t<HALF, uint16_t, float> StateValue;
+  StateValue* const state = static_cast<StateValue*>(p.state) + ro.state_at;
+  const uint32_t state_lane = 8 * g4 * KD + col;
   StatePair raw[4][8];
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t at = ro.state_at + (32 * s + 8 * g4 + i) * KD + col;
-      raw[s][i] = *reinterpret_cast<const StatePair*>(reinterpret_cast<const std::conditional_t<HALF, uint16_t, float>*>(p.state) + at);
-    }
+    for (int i = 0; i < 8; ++i) raw[s][i] = *reinterpret_cast<const StatePair*>(state + (32 * s + i) * KD + state_lane);
   const auto s0 = [&](int s, int j, int i) {
     if constexpr (HALF) return h2f((uint16_t)(raw[s][i] >> (16 * j)));
     else return raw[s][i][j];
@@ -273,15 +279,17 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(cons
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = min(16 * t + 4 * g4 + r, len - 1);
-      vw[t][r] = *reinterpret_cast<const uint32_t*>(ro.v + (int64_t)i * p.qkv_stride + col);
+      vw[t][r] = *reinterpret_cast<const uint32_t*>(ro.v + ((uint32_t)i * stride + col));
     }
+  uint32_t nw = 0;
   if constexpr (GATED) {
+    nw = *reinterpret_cast<const uint32_t*>(p.norm_w + col);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = min(16 * t + 4 * g4 + r, len - 1);
-        zw[t][r] = *reinterpret_cast<const uint32_t*>(ro.z + (int64_t)i * p.z_stride + col);
+        zw[t][r] = *reinterpret_cast<const uint32_t*>(ro.z + ((uint32_t)i * (uint32_t)p.z_stride + col));
       }
   }
   __builtin_amdgcn_sched_barrier(0);   // the loads stay where they stand
@@ -299,13 +307,13 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(cons
     }
     return add_xor32(add_xor16(ss));
   };
-  if (do_k) {
-    const float ss = stage(kp, lds.k);
-    if (g4 == 0) lds.kinv[16 * kt + c] = 1.0f / sqrtf(ss + 1e-6f);
-  }
-  if (do_q) {
-    const float ss = stage(qp, lds.q);
-    if (g4 == 0) lds.qinv[16 * kt + c] = p.scale / sqrtf(ss + 1e-6f);
+  if (!idle) {
+    const float ss = stage(kp, is_q ? lds.q : lds.k);
+    if (g4 == 0) (is_q ? lds.qinv : lds.kinv)[16 * kt + c] = (is_q ? p.scale : 1.0f) / sqrtf(ss + 1e-6f);
+    if constexpr (BOTH) {
+      const float qq = stage(qp, lds.q);
+      if (g4 == 0) lds.qinv[16 * kt + c] = p.scale / sqrtf(qq + 1e-6f);
+    }
   }
   // ---- a node's scalars: lane = node ----
   if (wave == 0) {
@@ -350,37 +358,54 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(cons
       kk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k_part(bi, s), y, kk, 0, 0, 0);
       qk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q_part(bi, s), y, qk, 0, 0, 0);
     }
-    const int j = 16 * bj + c;
+    const int j = 16 * bj + c, i0 = 16 * bi + 4 * g4;
     const double Gj = lds.G[j];
     const float kj = lds.kinv[j];
+    const f32x4 be = *reinterpret_cast<const f32x4*>(&lds.beta[i0]), ki = *reinterpret_cast<const f32x4*>(&lds.kinv[i0]);
+    const f32x4 qi = *reinterpret_cast<const f32x4*>(&lds.qinv[i0]);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * bi + 4 * g4 + r;
+      const int i = i0 + r;
       const bool on = (lds.mask[i] >> j & 1) && i < len;
       const float d = expf((float)(lds.G[i] - Gj)) * kj;
-      lds.P[i][j] = on ? lds.qinv[i] * d * qk[r] : 0.f;
-      lds.A[i][j] = on && i != j ? -lds.beta[i] * lds.kinv[i] * d * kk[r] : 0.f;
+      lds.P[i][j] = on ? qi[r] * d * qk[r] : 0.f;
+      lds.A[i][j] = on && i != j ? -be[r] * ki[r] * d * kk[r] : 0.f;
     }
   }
   lds_barrier();
 
-  // ---- the inverses of the diagonal blocks: wave = block, lane c = column ----
-  if (wave < tiles) {
-    float t[16];
+  // ---- the inverses of the diagonal blocks. X = -A_bb has X^16 = 0: (I - X)^-1 = (I + X)(I + X^2)(I + X^4)(I + X^8). x holds
+  // X in the accumulators' layout (x[r] = X[4 g4 + r][c], a B operand as it lies), y its transpose (y[r] = X[c][4 g4 + r], an A
+  // operand); each product of one with the other gives the next power of either. Rows past the tree's end are 0 in X. ----
+  const auto inverse = [&](int blk) {
+    f32x4 x, y = *reinterpret_cast<const f32x4*>(&lds.A[16 * blk + c][16 * blk + 4 * g4]);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t[i] = i == c ? 1.f : 0.f;
-    const int rows = min(16, len - 16 * wave);
+    for (int r = 0; r < 4; ++r) x[r] = lds.A[16 * blk + 4 * g4 + r][16 * blk + c];
+    f32x4 z = y;                                        // transposed: the A operand of the products with T
 #pragma unroll
-    for (int m = 0; m < 15; ++m) {   // t[m] is settled: its share of the rows below
-      if (m + 1 >= rows) break;
+    for (int r = 0; r < 4; ++r) z[r] += 4 * g4 + r == c ? 1.f : 0.f;
+    const int rows = len - 16 * blk;
 #pragma unroll
-      for (int i = m + 1; i < 16; ++i) t[i] = __builtin_fmaf(lds.A[16 * wave + i][16 * wave + m], t[m], t[i]);
+    for (int far = 2; far < 16; far <<= 1) {
+      if (far >= rows) break;
+      f32x4 x2 = {0.f, 0.f, 0.f, 0.f}, y2 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x2 = __builtin_amdgcn_mfma_f32_16x16x4f32(y[r], x[r], x2, 0, 0, 0);
+        y2 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], y[r], y2, 0, 0, 0);
+      }
+      x = x2;
+      y = y2;
+      f32x4 z2 = z;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) z2 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], z[r], z2, 0, 0, 0);
+      z = z2;
     }
-    if (g4 == 0) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) lds.T[wave][i][c] = t[i];
-    }
-  }
+    return z;
+  };
+  f32x4 t0 = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (NT == 1) t0 = inverse(0);
+  else if (wave < tiles) lds.T[wave][lane] = inverse(wave);
 
   // ---- S0^T k and S0^T q of every node, the wave's columns ----
   f32x4 u[NT][2], o[NT][2];
@@ -410,6 +435,7 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(cons
           o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf, part[j][w], o[t][j], 0, 0, 0);
         }
     }
+    __builtin_amdgcn_sched_barrier(0);   // the parts of one step at a time in registers
   }
   // ---- R, and the state's part of the outputs ----
 #pragma unroll
@@ -429,7 +455,7 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(cons
       }
     }
   }
-  lds_barrier();
+  if constexpr (NT > 1) lds_barrier();
 
   // ---- U, block by block, and the outputs ----
 #pragma unroll
@@ -443,7 +469,7 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(cons
 #pragma unroll
         for (int j = 0; j < 2; ++j) u[b][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], u[t][j][r], u[b][j], 0, 0, 0);
     }
-    const f32x4 a = *reinterpret_cast<const f32x4*>(&lds.T[b][c][4 * g4]);
+    const f32x4 a = NT == 1 ? t0 : lds.T[b][lane];
     f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -486,8 +512,8 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(cons
   }
 
   // ---- gated norm, outputs ----
-  float nw[2] = {0.f, 0.f};
-  if constexpr (GATED) unpack2(*reinterpret_cast<const uint32_t*>(p.norm_w + col), nw[0], nw[1]);
+  float w2[2];
+  unpack2(nw, w2[0], w2[1]);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (t >= tiles) break;
@@ -501,14 +527,14 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(cons
         float z[2];
         unpack2(zw[t][r], z[0], z[1]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) y[j] *= rs * nw[j] * siluf_(z[j]);
+        for (int j = 0; j < 2; ++j) y[j] *= rs * w2[j] * siluf_(z[j]);
       }
-      if (i < len) *reinterpret_cast<uint32_t*>(ro.out + (int64_t)i * p.HV * KD + col) = pack_bf16x2(y[0], y[1]);
+      if (i < len) *reinterpret_cast<uint32_t*>(ro.out + ((uint32_t)i * (uint32_t)(p.HV * KD) + col)) = pack_bf16x2(y[0], y[1]);
     }
   }
 
   // ---- the committed chain moves the state: u scaled, split as the state was, times k^T read from LDS transposed ----
-  if (ro.done > 0) {
+  if (MOVES && ro.done > 0) {
     const float ec = lds.eG[ro.done - 1];
     constexpr int NP = (NT + 1) / 2;     // pairs of tiles: a product takes 32 nodes, the lane's own 4 of either tile
     bf16x8 up[NP][2][3];
@@ -559,12 +585,9 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 3 : 2) void gdn_tree_kernel(cons
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int64_t at = ro.state_at + (32 * s + 8 * g4 + 4 * hh + r) * KD + col;
-          if constexpr (HALF)
-            *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.state) + at) =
-                (uint32_t)f2h(acc[0][r]) | ((uint32_t)f2h(acc[1][r]) << 16);
-          else
-            *reinterpret_cast<f32x2*>(static_cast<float*>(p.state) + at) = (f32x2){acc[0][r], acc[1][r]};
+          StateValue* const at = state + (32 * s + 4 * hh + r) * KD + state_lane;
+          if constexpr (HALF) *reinterpret_cast<uint32_t*>(at) = (uint32_t)f2h(acc[0][r]) | ((uint32_t)f2h(acc[1][r]) << 16);
+          else *reinterpret_cast<f32x2*>(at) = (f32x2){acc[0][r], acc[1][r]};
         }
       }
   }
@@ -588,6 +611,8 @@ extern "C" int hsg_gdn_tree_step(const void* qkv, int64_t qkv_stride, int32_t q_
   if (!qkv || !a || !b || !A_log || !dt_bias || !state || !slots || !lens || !offsets || !masks || !out ||
       (z && !norm_w))
     return HSG_ERR_ARG;
+  // a row's values are addressed by 32-bit byte offsets
+  if (qkv_stride < 0 || qkv_stride >= (1 << 24) || z_stride >= (1 << 24) || HV >= (1 << 16)) return HSG_ERR_SHAPE;
   if (q_off < 0 || k_off < 0 || v_off < 0 || ab_stride < HV || (z && z_stride < (int64_t)HV * KD)) return HSG_ERR_ARG;
   if (qkv_stride % 8 || q_off % 8 || k_off % 8 || v_off % 8 || !aligned(qkv, 16) || !aligned(state, 16) ||
       !aligned(out, 4) || (z && (z_stride % 2 || !aligned(z, 4) || !aligned(norm_w, 4))))
@@ -608,8 +633,13 @@ extern "C" int hsg_gdn_tree_step(const void* qkv, int64_t qkv_stride, int32_t q_
   };
   const auto by_type = [&](auto nt) {
     constexpr int NT = decltype(nt)::value;
-    if (state_dtype == HSG_STATE_F16) z ? launch(gdn_tree_kernel<NT, true, true>) : launch(gdn_tree_kernel<NT, true, false>);
-    else z ? launch(gdn_tree_kernel<NT, false, true>) : launch(gdn_tree_kernel<NT, false, false>);
+    const auto by_state = [&](auto half) {
+      constexpr bool HALF = decltype(half)::value;
+      if (commits) z ? launch(gdn_tree_kernel<NT, HALF, true, true>) : launch(gdn_tree_kernel<NT, HALF, false, true>);
+      else z ? launch(gdn_tree_kernel<NT, HALF, true, false>) : launch(gdn_tree_kernel<NT, HALF, false, false>);
+    };
+    if (state_dtype == HSG_STATE_F16) by_state(std::true_type{});
+    else by_state(std::false_type{});
   };
   if (max_nodes <= 16) by_type(std::integral_constant<int, 1>{});
   else if (max_nodes <= 32) by_type(std::integral_constant<int, 2>{});
