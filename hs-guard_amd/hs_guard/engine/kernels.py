@@ -338,50 +338,71 @@ class DraftTrees(NamedTuple):
     max_nodes: int = HSG_TREE_MAX_NODES     # bound on every row's nodes; smaller bounds take smaller tiles
 
 
-def _index_tensors(like, *tensors):
-    """The index tensors (None skipped) are contiguous int64 on the device of ``like``."""
+_I64 = torch.int64
+_current_device = torch._C._cuda_getDevice
+
+
+def _device_of(*tensors):
+    """The index of the one GPU that the tensors (None skipped) are on."""
+    index = tensors[0].get_device()
+    if index < 0:
+        raise AssertionError("HS-Guard kernels take GPU tensors")
     for t in tensors:
-        _require(t is None or (t.dtype is torch.int64 and t.is_contiguous() and t.device == like.device),
-                 "index tensors must be contiguous int64 on the operands' device")
+        if t is not None and t.get_device() != index:
+            raise AssertionError("tensors must be on one GPU")
+    return index
 
 
-def _tree_rows(trees, slots, tokens, like):
-    """Checks of a batch of trees over ``tokens`` packed tokens; returns its rows."""
-    n = slots.shape[0]
-    _index_tensors(like, slots, *trees[:5])
-    _require(slots.dim() == 1 and trees.offsets.shape == (n,) and trees.lens.shape == (n,)
-             and (trees.commits is None or trees.commits.shape == (n,)), "offsets, lens, commits and slots must be [n]")
-    _require(trees.masks.shape == (tokens,), "masks must be [T], one for each packed token")
-    _require(1 <= trees.max_nodes <= HSG_TREE_MAX_NODES, f"max_nodes must be in [1, {HSG_TREE_MAX_NODES}]")
-    return n
+def _index_tensors(*tensors):
+    """The index tensors (None skipped) are contiguous int64."""
+    for t in tensors:
+        if t is not None and (t.dtype is not _I64 or not t.is_contiguous()):
+            raise AssertionError("index tensors must be contiguous int64")
 
 
-def _packed_rows(t, width):
-    """t's rows [T, ...] lie ``stride(0)`` apart, each one's ``width`` values next to one another."""
-    _require(t.dtype is torch.bfloat16, "bf16 tensors expected")
+def _tree_rows(trees, slots, tokens):
+    """Checks a batch of trees over ``tokens`` packed tokens; returns its rows."""
+    offsets, lens, commits, _, masks, most = trees
+    _index_tensors(slots, offsets, lens, commits, masks)
+    shape = slots.shape
+    if len(shape) != 1 or offsets.shape != shape or lens.shape != shape or (commits is not None
+                                                                           and commits.shape != shape):
+        raise AssertionError("offsets, lens, commits and slots must be [n]")
+    if masks.shape != (tokens,):
+        raise AssertionError("masks must be [T], one for each packed token")
+    if not 1 <= most <= HSG_TREE_MAX_NODES:
+        raise AssertionError(f"max_nodes must be in [1, {HSG_TREE_MAX_NODES}]")
+    return shape[0]
+
+
+def _packed_rows(t, tokens, width):
+    """t [tokens, ...] bf16 holds each token's ``width`` values next to one another: how far apart its tokens lie."""
+    if t.dtype is not torch.bfloat16 or t.shape[0] != tokens or t.numel() != tokens * width:
+        raise AssertionError(f"[{tokens}, {width}] bf16 values expected, got {list(t.shape)} of {t.dtype}")
+    if t.is_contiguous():
+        return width
     inner = 1
     for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-        _require(size == 1 or stride == inner, "a token's values must be contiguous")
+        if size != 1 and stride != inner:
+            raise AssertionError("a token's values must be contiguous")
         inner *= size
-    _require(inner == width, f"{width} values a token expected, got {inner}")
-    _require(t.shape[0] <= 1 or t.stride(0) >= width, "tokens must not overlap")
-    return t.stride(0) if t.shape[0] > 1 else width
+    stride = t.stride(0) if tokens > 1 else width
+    if stride < width:
+        raise AssertionError("tokens must not overlap")
+    return stride
 
 
-class _on:
-    """The device of ``t`` as the current one: a launch goes to the current device, whatever its stream."""
-
-    def __init__(self, t):
-        self.device = t.device.index
-
-    def __enter__(self):
-        self.before = torch._C._cuda_getDevice()
-        if self.before != self.device:
-            torch._C._cuda_setDevice(self.device)
-
-    def __exit__(self, *exc):
-        if self.before != self.device:
-            torch._C._cuda_setDevice(self.before)
+def _launch(name, device, *args):
+    """The entry point on the device's current stream, with that device as the current one: a launch goes to the current
+    device, whatever its stream."""
+    call = getattr(calls(), name)
+    if _current_device() == device:
+        rc = call(*args, _current_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = call(*args, _current_stream(device))
+    if rc:
+        check(rc, name)
 
 
 def draft_tree_maps(parents, lens, starts, commits=None, max_nodes=HSG_TREE_MAX_NODES):
@@ -390,21 +411,19 @@ def draft_tree_maps(parents, lens, starts, commits=None, max_nodes=HSG_TREE_MAX_
     int64: nodes of each row, tokens its session holds, leading nodes to commit. A row that is no tree (a parent that does
     not come before its child, more than ``max_nodes`` nodes or more than the buffer holds, commits that are no chain from
     the session's last token) comes back with lens and commits 0. pos and masks of tokens of no row are 0."""
-    _gpu(parents, lens, starts, commits)
-    _index_tensors(parents, parents, lens, starts, commits)
-    n = lens.shape[0]
-    _require(parents.dim() == 1 and lens.dim() == 1 and starts.shape == (n,) and (commits is None or commits.shape == (n,)),
-             "parents must be [T]; lens, starts and commits [n]")
-    _require(1 <= max_nodes <= HSG_TREE_MAX_NODES, f"max_nodes must be in [1, {HSG_TREE_MAX_NODES}]")
-    total = parents.shape[0]
+    device = _device_of(parents, lens, starts, commits)
+    _index_tensors(parents, lens, starts, commits)
+    shape = lens.shape
+    if parents.dim() != 1 or len(shape) != 1 or starts.shape != shape or (commits is not None and commits.shape != shape):
+        raise AssertionError("parents must be [T]; lens, starts and commits [n]")
+    if not 1 <= max_nodes <= HSG_TREE_MAX_NODES:
+        raise AssertionError(f"max_nodes must be in [1, {HSG_TREE_MAX_NODES}]")
     offsets, lens_out = torch.empty_like(lens), torch.empty_like(lens)
-    commits_out = None if commits is None else torch.empty_like(commits)
+    commits_out = None if commits is None else torch.empty_like(lens)
     pos, masks = torch.empty_like(parents), torch.empty_like(parents)
-    with _on(parents):
-        rc = calls().hsg_tree_maps(_ptr(parents), total, _ptr(lens), _ptr(starts), _ptr(commits), n, max_nodes,
-                                   _ptr(offsets), _ptr(lens_out), _ptr(commits_out), _ptr(pos), _ptr(masks),
-                                   _stream(parents))
-    check(rc, "hsg_tree_maps")
+    _launch("hsg_tree_maps", device, parents.data_ptr(), parents.shape[0], lens.data_ptr(), starts.data_ptr(),
+            _ptr(commits), shape[0], max_nodes, offsets.data_ptr(), lens_out.data_ptr(), _ptr(commits_out), pos.data_ptr(),
+            masks.data_ptr())
     return DraftTrees(offsets, lens_out, commits_out, pos, masks, max_nodes)
 
 
@@ -413,19 +432,17 @@ def tree_conv_silu(qkv, pool, weight, slots, trees):
     (rows may lie further apart), pool [S, 3, C] bf16 (one layer), weight [C, 1, 4] bf16. Returns [T, C] bf16; tokens of no
     row are not written. Rows that commit move their history in ``pool`` and need slots of their own."""
     total, c = qkv.shape
-    _gpu(qkv, pool, weight, slots)
-    stride = _packed_rows(qkv, c)
+    device = _device_of(qkv, pool, weight, slots, *trees[:5])
+    stride = _packed_rows(qkv, total, c)
     _bf16_in(pool, weight)
     ks = weight.shape[-1]
-    _require(pool.dim() == 3 and pool.shape[1:] == (ks - 1, c) and weight.numel() == c * ks,
-             "tree_conv_silu: pool [S, K-1, C], weight [C, 1, K]")
-    n = _tree_rows(trees, slots, total, qkv)
-    out = torch.empty((total, c), dtype=qkv.dtype, device=qkv.device)
-    with _on(qkv):
-        rc = calls().hsg_tree_conv_silu(_ptr(qkv), stride, _ptr(pool), pool.shape[0], _ptr(weight), ks, _ptr(slots),
-                                        _ptr(trees.lens), _ptr(trees.offsets), _ptr(trees.commits), _ptr(trees.masks), n,
-                                        trees.max_nodes, c, _ptr(out), c, _stream(qkv))
-    check(rc, "hsg_tree_conv_silu")
+    if pool.dim() != 3 or pool.shape[1] != ks - 1 or pool.shape[2] != c or weight.numel() != c * ks:
+        raise AssertionError("tree_conv_silu: pool [S, K-1, C], weight [C, 1, K]")
+    n = _tree_rows(trees, slots, total)
+    out = qkv.new_empty((total, c))
+    _launch("hsg_tree_conv_silu", device, qkv.data_ptr(), stride, pool.data_ptr(), pool.shape[0], weight.data_ptr(), ks,
+            slots.data_ptr(), trees.lens.data_ptr(), trees.offsets.data_ptr(), _ptr(trees.commits), trees.masks.data_ptr(),
+            n, trees.max_nodes, c, out.data_ptr(), c)
     return out
 
 
@@ -438,33 +455,30 @@ def gdn_tree_step(packed, key_dim, heads, head_k, value_heads, head_v, a, b, A_l
     that commit move their state and need slots of their own; no other state is written."""
     total = packed.shape[0]
     hvv = value_heads * head_v
-    _gpu(packed, a, b, A_log, dt_bias, state, slots, z, norm_weight)
-    stride = _packed_rows(packed, 2 * key_dim + hvv)
-    _require(key_dim == heads * head_k, "key_dim must be heads * head_k")
-    _require(a.shape == (total, value_heads) and b.shape == a.shape, "a and b must be [T, HV]")
-    ab = _packed_rows(a, value_heads)
-    _require(_packed_rows(b, value_heads) == ab, "a and b must have one row stride")
+    device = _device_of(packed, a, b, A_log, dt_bias, state, slots, z, norm_weight, *trees[:5])
+    stride = _packed_rows(packed, total, 2 * key_dim + hvv)
+    ab = _packed_rows(a, total, value_heads)
+    if key_dim != heads * head_k or _packed_rows(b, total, value_heads) != ab:
+        raise AssertionError("key_dim must be heads * head_k, and a and b have one row stride")
     _bf16_in(A_log, dt_bias)
-    _require(A_log.numel() == value_heads and dt_bias.numel() == value_heads, "A_log and dt_bias must be [HV]")
-    _require(state.dtype in _STATE_CODES and state.is_contiguous() and state.shape[1:] == (value_heads, head_k, head_v),
-             "state must be contiguous [S, HV, K, V], float32 or float16")
-    _require((z is None) == (norm_weight is None), "the gated norm takes z and norm_weight")
+    if A_log.numel() != value_heads or dt_bias.numel() != value_heads:
+        raise AssertionError("A_log and dt_bias must be [HV]")
+    if state.dtype not in _STATE_CODES or not state.is_contiguous() or state.shape[1:] != (value_heads, head_k, head_v):
+        raise AssertionError("state must be contiguous [S, HV, K, V], float32 or float16")
+    if (z is None) != (norm_weight is None):
+        raise AssertionError("the gated norm takes z and norm_weight")
     z_stride = 0
     if z is not None:
-        _require(z.shape[0] == total, "z must be [T, HV*V]")
-        z_stride = _packed_rows(z, hvv)
+        z_stride = _packed_rows(z, total, hvv)
         _bf16_in(norm_weight)
         _require(norm_weight.numel() == head_v, "norm_weight must be [V]")
-    n = _tree_rows(trees, slots, total, packed)
-    out = torch.empty((total, hvv), dtype=packed.dtype, device=packed.device)
-    scale = head_k ** -0.5 if scale is None else scale
-    with _on(packed):
-        rc = calls().hsg_gdn_tree_step(
-            _ptr(packed), stride, 0, key_dim, 2 * key_dim, _ptr(a), _ptr(b), ab, _ptr(A_log), _ptr(dt_bias), _ptr(state),
-            _STATE_CODES[state.dtype], state.shape[0], _ptr(slots), _ptr(trees.lens), _ptr(trees.offsets),
-            _ptr(trees.commits), _ptr(trees.masks), n, trees.max_nodes, heads, value_heads, head_k, head_v, float(scale),
-            _ptr(z), z_stride, _ptr(norm_weight), float(eps), _ptr(out), _stream(packed))
-    check(rc, "hsg_gdn_tree_step")
+    n = _tree_rows(trees, slots, total)
+    out = packed.new_empty((total, hvv))
+    _launch("hsg_gdn_tree_step", device, packed.data_ptr(), stride, 0, key_dim, 2 * key_dim, a.data_ptr(), b.data_ptr(), ab,
+            A_log.data_ptr(), dt_bias.data_ptr(), state.data_ptr(), _STATE_CODES[state.dtype], state.shape[0],
+            slots.data_ptr(), trees.lens.data_ptr(), trees.offsets.data_ptr(), _ptr(trees.commits), trees.masks.data_ptr(),
+            n, trees.max_nodes, heads, value_heads, head_k, head_v, head_k ** -0.5 if scale is None else float(scale),
+            _ptr(z), z_stride, _ptr(norm_weight), float(eps), out.data_ptr())
     return out
 
 
@@ -478,33 +492,31 @@ def tree_ring_attention(q, ring_k, ring_v, new_k, value, gate, ring_pos, slots, 
     tensor of hsg_tree_attention_workspace_bytes, which calls of few rows use (allocated per call when None)."""
     total, hq, d = q.shape
     hkv = new_k.shape[1]
-    _gpu(q, ring_k, ring_v, new_k, value, gate, ring_pos, slots, starts, workspace)
-    _require(hkv > 0 and hq % hkv == 0, "query heads must be a multiple of the kv heads")
+    device = _device_of(q, ring_k, ring_v, new_k, value, gate, ring_pos, slots, starts, workspace, *trees[:5])
+    if hkv == 0 or hq % hkv:
+        raise AssertionError("query heads must be a multiple of the kv heads")
     groups = hq // hkv
-    _require(new_k.shape == (total, hkv, d) and value.numel() == total * hkv * d and value.shape[0] == total,
-             "new_k and value must be [T, Hkv, D]")
-    qs, ks, vs = _packed_rows(q, hq * d), _packed_rows(new_k, hkv * d), _packed_rows(value, hkv * d)
-    gs = 0
-    if gate is not None:
-        _require(gate.shape[0] == total, "gate must be [T, Hq*2D]")
-        gs = _packed_rows(gate, hq * 2 * d)
+    qs, ks, vs = _packed_rows(q, total, hq * d), _packed_rows(new_k, total, hkv * d), _packed_rows(value, total, hkv * d)
+    gs = 0 if gate is None else _packed_rows(gate, total, hq * 2 * d)
     _bf16_in(ring_k, ring_v)
-    _require(ring_k.dim() == 4 and ring_k.shape[1:] == (hkv, window + 1, d) and ring_v.shape == ring_k.shape,
-             "ring_k and ring_v must be [S, Hkv, W+1, D]")
-    _require(ring_pos.shape == (ring_k.shape[0], window + 1), "ring_pos must be [S, W+1]")
-    _index_tensors(q, ring_pos, starts)
-    n = _tree_rows(trees, slots, total, q)
-    _require(starts.shape == (n,), "starts must be [n]")
-    out = torch.empty((total, hq * d), dtype=q.dtype, device=q.device)
+    rings = ring_k.shape
+    if len(rings) != 4 or rings[1:] != (hkv, window + 1, d) or ring_v.shape != rings:
+        raise AssertionError("ring_k and ring_v must be [S, Hkv, W+1, D]")
+    if ring_pos.shape != (rings[0], window + 1):
+        raise AssertionError("ring_pos must be [S, W+1]")
+    _index_tensors(ring_pos, starts)
+    n = _tree_rows(trees, slots, total)
+    _require(starts.shape == slots.shape, "starts must be [n]")
+    out = q.new_empty((total, hq * d))
+    most = trees.max_nodes
     if workspace is None:
-        need = lib().hsg_tree_attention_workspace_bytes(n, hkv, groups, trees.max_nodes)
+        need = lib().hsg_tree_attention_workspace_bytes(n, hkv, groups, most)
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    with _on(q):
-        rc = calls().hsg_tree_attention(
-            _ptr(q), qs, groups * d, d, _ptr(ring_k), _ptr(ring_v), ring_k.shape[0], window, _ptr(new_k), ks, d,
-            _ptr(value), vs, d, _ptr(gate), gs, groups * 2 * d, 2 * d, d, _ptr(ring_pos), _ptr(slots), _ptr(starts),
-            _ptr(trees.lens), _ptr(trees.offsets), _ptr(trees.commits), _ptr(trees.masks), n, trees.max_nodes, hkv, groups,
-            d, float(scale), _ptr(out), hq * d, groups * d, d, _ptr(workspace), 0 if workspace is None else
-            workspace.numel(), _stream(q))
-    check(rc, "hsg_tree_attention")
+    else:
+        _require(workspace.dtype is torch.uint8 and workspace.is_contiguous(), "workspace must be contiguous uint8")
+    _launch("hsg_tree_attention", device, q.data_ptr(), qs, groups * d, d, ring_k.data_ptr(), ring_v.data_ptr(), rings[0],
+            window, new_k.data_ptr(), ks, d, value.data_ptr(), vs, d, _ptr(gate), gs, groups * 2 * d, 2 * d, d,
+            ring_pos.data_ptr(), slots.data_ptr(), starts.data_ptr(), trees.lens.data_ptr(), trees.offsets.data_ptr(),
+            _ptr(trees.commits), trees.masks.data_ptr(), n, most, hkv, groups, d, float(scale), out.data_ptr(), hq * d,
+            groups * d, d, _ptr(workspace), 0 if workspace is None else workspace.numel())
     return out
