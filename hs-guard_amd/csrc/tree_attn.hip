@@ -213,7 +213,7 @@ struct KeyStage {
 template <int T, int KW, bool STAGED>
 struct TreeAttnLds {
   static constexpr int QW = NW / KW;
-  static constexpr int STAGES = STAGED ? 4 : 1;
+  static constexpr int STAGES = STAGED ? 2 : 1;
   union {
     struct {
       u32x4 q[STAGED ? 1 : QW * T][D / 32][64];   // the queries' operands, in the order of the lanes
@@ -229,7 +229,7 @@ struct TreeAttnLds {
 };
 
 template <int T, int KW, bool STAGED>
-__global__ __launch_bounds__(64 * NW, T == 1 ? 2 : 1) void tree_attn_kernel(const TreeAttnParams p) {
+__global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_kernel(const TreeAttnParams p) {
   constexpr int QW = NW / KW;
   constexpr int ROWS = 16 * T * QW;     // query rows of the workgroup
   __shared__ __align__(16) TreeAttnLds<T, KW, STAGED> lds;
@@ -438,8 +438,7 @@ __global__ __launch_bounds__(64 * NW, T == 1 ? 2 : 1) void tree_attn_kernel(cons
       add_values(1, vr[1], pb);
     }
   } else {
-    // every wave needs every block: blocks pass through LDS, three ahead of the one at work
-    constexpr int AHEAD = TreeAttnLds<T, KW, STAGED>::STAGES - 1;
+    // every wave needs every block: blocks pass through LDS, the next one on its way while one is at work
     constexpr int EACH = 2 * KB * D * 2 / 1024 / NW;      // a wave's loads of a block
     const auto fetch = [&](int b, int stage) __attribute__((always_inline)) {
       const bool ring = b < RB;
@@ -457,26 +456,14 @@ __global__ __launch_bounds__(64 * NW, T == 1 ? 2 : 1) void tree_attn_kernel(cons
         load_lds16(vb, 2 * v_off, __builtin_amdgcn_readfirstlane(to + (uint32_t)offsetof(KeyStage, v) + 1024 * o));
       }
     };
-    int ahead = next_block(split - step);                 // the next block to fetch
-    int b = ahead;
-    int stage = 0, fetched = 0;                           // blocks fetched and not yet worked on, after b
-    for (; fetched < AHEAD && ahead < n_blocks; ++fetched) {
-      fetch(ahead, fetched);
-      ahead = next_block(ahead);
-    }
+    int b = next_block(split - step), stage = 0;
+    if (b < n_blocks) fetch(b, 0);
     while (b < n_blocks) {
-      // the oldest block has landed: at most the later ones' loads are outstanding
-      if (fetched >= 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * EACH) : "memory");
-      else if (fetched == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(EACH) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // the block has landed
       __builtin_amdgcn_s_barrier();                       // for every wave; and the block before is read no more
       asm volatile("" ::: "memory");
-      --fetched;
-      if (ahead < n_blocks) {
-        fetch(ahead, (stage + AHEAD) % (AHEAD + 1));
-        ahead = next_block(ahead);
-        ++fetched;
-      }
+      const int b_next = next_block(b);
+      if (b_next < n_blocks) fetch(b_next, stage ^ 1);
       if (tiles > 0) {
         const KeyStage& ks_ = lds.stage[stage];
         f32x4 S[T][2];
@@ -502,8 +489,8 @@ __global__ __launch_bounds__(64 * NW, T == 1 ? 2 : 1) void tree_attn_kernel(cons
           add_values(hh, vr, pb);
         }
       }
-      b = next_block(b);
-      stage = (stage + 1) % (AHEAD + 1);
+      b = b_next;
+      stage ^= 1;
     }
   }
 
