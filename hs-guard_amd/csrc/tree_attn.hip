@@ -96,6 +96,10 @@ __device__ __forceinline__ bool tree_keys(const TreeAttnParams& p, int n, int h,
 
 __device__ __forceinline__ bf16x8 as_bf16x8(u32x4 w) { return __builtin_bit_cast(bf16x8, w); }
 __device__ __forceinline__ u32x4 load16(const uint16_t* p) { return *reinterpret_cast<const u32x4*>(p); }
+// 16 bytes at byte `off` of a base that is the same for all lanes: its address takes one register of a lane
+__device__ __forceinline__ u32x4 load16_at(const uint16_t* base, uint32_t off) {
+  return *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + off);
+}
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // node i's ancestors and itself
@@ -167,16 +171,23 @@ __device__ __forceinline__ bool all_finite(const float (&y)[ND]) {
   return odd == 0.f;
 }
 
+// The gate of ND values (dims d0 ..) of query `row`
+template <int N8>
+__device__ __forceinline__ void load_gate(const TreeAttnParams& p, const TreeKeys& ro, int row, int d0, u32x4 (&gw)[N8]) {
+  if (!ro.gate) return;
+  const int l = row / p.G, g = row - l * p.G;
+  const uint16_t* src = ro.gate + l * p.g_sl + g * p.g_sg + d0;
+#pragma unroll
+  for (int e = 0; e < N8; ++e) gw[e] = load16(src + 8 * e);
+}
+
 // ND normalised values of query `row`, gated and stored (dims d0 ..)
 template <int ND>
-__device__ __forceinline__ void store_gated(const TreeAttnParams& p, const TreeKeys& ro, int row, int d0, float (&y)[ND]) {
+__device__ __forceinline__ void store_gated(const TreeAttnParams& p, const TreeKeys& ro, int row, int d0, float (&y)[ND],
+                                            const u32x4 (&gw)[ND / 8]) {
   const int l = row / p.G, g = row - l * p.G;
   uint16_t* dst = ro.out + l * p.o_sl + g * p.o_sg + d0;
   if (ro.gate) {
-    const uint16_t* src = ro.gate + l * p.g_sl + g * p.g_sg + d0;
-    u32x4 gw[ND / 8];
-#pragma unroll
-    for (int e = 0; e < ND / 8; ++e) gw[e] = load16(src + 8 * e);
 #pragma unroll
     for (int e = 0; e < ND / 8; ++e) {
       float gt[8];
@@ -205,9 +216,11 @@ __device__ __forceinline__ void load_lds16(const void* base, uint32_t off, uint3
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
 }
 
+// Rows of 512 bytes, each loaded whole. The 16-byte pieces of a key are permuted by its number (piece pc of row r at pc ^ r %
+// 16), so that the scores' operand, one piece of 16 rows, spreads over the banks; of a value 16 pieces of a row are read.
 struct KeyStage {
-  u32x4 k[2][D / 32][64];   // A operands of the scores, in the order of the lanes
-  uint16_t v[KB][D];        // row by row
+  uint16_t k[KB][D];
+  uint16_t v[KB][D];
 };
 
 template <int T, int KW, bool STAGED>
@@ -222,6 +235,7 @@ struct TreeAttnLds {
     f32x4 o[KW > 1 ? NW : 1][16][64];             // a tile's partial sums of every wave
   };
   int kp[W_MAX + MOST];       // places of the ring's keys before the start; then the nodes' depths
+  uint64_t mask[MOST];        // the nodes' ancestors and themselves
   uint32_t flags[BLOCKS];     // bit 0: some query may see a key of the block; 1: all see all
   float ml[NW][T][16][2];
   uint32_t odd[QW * T];       // query rows with a result that is not finite
@@ -257,18 +271,18 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
   const int l_hi = (min(r_wg + ROWS, M) - 1) / G;           // last node of the workgroup
   const int RB = W / KB;
   const int n_blocks = RB + l_hi / KB + 1;
+  const int step = KW * p.splits;
+  const int b_first = wk + KW * split;                      // the first of the wave's blocks
 
   // ---- queries, and places of the keys ----
   bf16x8 qr[STAGED ? T : 1][D / 32];
-  uint64_t mask[T];
-  int depth[T];
+  int node[T];
 #pragma unroll
   for (int t = 0; t < T; ++t) {
     const int row = min(r_lo + 16 * t + c, M - 1);           // past the valid rows: the last one again, not stored
     const int l = row / G;
     const uint16_t* src = ro.q + l * p.q_sl + (row - l * G) * p.q_sg + 8 * g4;
-    mask[t] = mask_of(ro.masks, l);
-    depth[t] = depth_of(ro.masks, l);
+    node[t] = l;
     if constexpr (STAGED) {
 #pragma unroll
       for (int ks = 0; ks < D / 32; ++ks) qr[t][ks] = as_bf16x8(load16(src + 32 * ks));
@@ -289,15 +303,16 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
     }
   }
   if (threadIdx.x < MOST) {
-    const int i = min((int)threadIdx.x, len - 1);
-    lds.kp[W_MAX + threadIdx.x] = depth_of(ro.masks, i);
+    const uint64_t mask = mask_of(ro.masks, min((int)threadIdx.x, len - 1));
+    lds.mask[threadIdx.x] = mask;
+    lds.kp[W_MAX + threadIdx.x] = (int)__popcll(mask) - 1;
   }
   if (threadIdx.x < QW * T) lds.odd[threadIdx.x] = 0u;
   __syncthreads();
 
   // ---- the wave's key blocks ----
-  const float sl2 = p.scale * LOG2E;
-  float m[T], sum[T];
+  const float sl2 = fmaxf(fabsf(p.scale) * LOG2E, 1e-37f);   // (not 0: a masked score is -inf)
+  float m[T], sum[T];   // (sum: of the lane's own keys)
   f32x4 O[T][2][8];
 #pragma unroll
   for (int t = 0; t < T; ++t) {
@@ -308,35 +323,39 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
 #pragma unroll
       for (int i = 0; i < 8; ++i) O[t][hh][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  const int step = KW * p.splits;
-  const auto next_block = [&](int b) {   // the next of the wave's blocks that a query may see
-    for (b += step; b < n_blocks; b += step)
-      if (b >= RB || (__builtin_amdgcn_readfirstlane(lds.flags[b]) & 1u)) break;
-    return b;
-  };
+  // bit b: the wave takes block b, which some query may see; and of these the ones that all see whole
+  uint32_t rest = 0u, whole;
+  {
+    const uint32_t f = lane < RB ? lds.flags[lane] : 0u;
+    const uint32_t some = (uint32_t)__ballot((f & 1u) != 0u) | (~0u << RB);
+    whole = (uint32_t)__ballot((f & 2u) != 0u);
+    for (int b = b_first; b < n_blocks; b += step) rest |= some & (1u << b);
+    if (tiles == 0 && KW > 1) rest = 0u;
+  }
   // probabilities of block b for the scores S, rounded; the accumulators follow a maximum that has moved
   const auto softmax = [&](int b, f32x4 (&S)[T][2], bf16x8 (&pb)[T]) __attribute__((always_inline)) {
     const bool ring = b < RB;
-    const bool full = ring && (__builtin_amdgcn_readfirstlane(lds.flags[b]) & 2u);
     float top[T];
     bool move = false;
-    if (full) {
+    if (p.scale < 0.f) {
 #pragma unroll
       for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) S[t][e >> 2][e & 3] *= sl2;
-    } else {
+        for (int e = 0; e < 8; ++e) S[t][e >> 2][e & 3] = -S[t][e >> 2][e & 3];
+    }
+    if (!(whole >> b & 1u)) {
       const int at = (ring ? b * KB : W_MAX + (b - RB) * KB) + 4 * g4;
       i32x4 place[2];
       place[0] = *reinterpret_cast<const i32x4*>(&lds.kp[at]);
       place[1] = *reinterpret_cast<const i32x4*>(&lds.kp[at + 16]);
 #pragma unroll
       for (int t = 0; t < T; ++t) {
-        const uint32_t bits = ring ? ~0u : (uint32_t)(mask[t] >> ((b - RB) * KB)) >> (4 * g4);
+        const int floor = lds.kp[W_MAX + node[t]] - W;
+        const uint32_t bits = ring ? ~0u : (uint32_t)(lds.mask[node[t]] >> ((b - RB) * KB)) >> (4 * g4);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const bool ok = place[e >> 2][e & 3] > depth[t] - W && (bits >> (16 * (e >> 2) + (e & 3)) & 1u);
-          S[t][e >> 2][e & 3] = ok ? S[t][e >> 2][e & 3] * sl2 : -INFINITY;
+          const bool ok = place[e >> 2][e & 3] > floor && (bits >> (16 * (e >> 2) + (e & 3)) & 1u);
+          S[t][e >> 2][e & 3] = ok ? S[t][e >> 2][e & 3] : -INFINITY;
         }
       }
     }
@@ -344,7 +363,7 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
     for (int t = 0; t < T; ++t) {
       top[t] = fmaxf(fmaxf(fmaxf(S[t][0][0], S[t][0][1]), fmaxf(S[t][0][2], S[t][0][3])),
                      fmaxf(fmaxf(S[t][1][0], S[t][1][1]), fmaxf(S[t][1][2], S[t][1][3])));
-      top[t] = max_pair32(max_pair16(top[t]));
+      top[t] = max_pair32(max_pair16(top[t])) * sl2;
       move |= top[t] > m[t] + SLACK;
     }
     if (__any(move)) {
@@ -366,7 +385,8 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
       u32x4 w;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p0 = exp2_fast(S[t][i >> 1][2 * (i & 1)] - base), p1 = exp2_fast(S[t][i >> 1][2 * (i & 1) + 1] - base);
+        const float p0 = exp2_fast(__builtin_fmaf(S[t][i >> 1][2 * (i & 1)], sl2, -base));
+        const float p1 = exp2_fast(__builtin_fmaf(S[t][i >> 1][2 * (i & 1) + 1], sl2, -base));
         sum[t] += p0 + p1;
         w[i] = pack_bf16x2(p0, p1);
       }
@@ -398,14 +418,14 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
       const int last = ring ? KB - 1 : len - 1 - (b - RB) * KB;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const uint32_t off = (uint32_t)min(16 * kt + c, last) * st + 8 * g4;
+        const uint32_t off = 2 * ((uint32_t)min(16 * kt + c, last) * st + 8 * g4);
 #pragma unroll
-        for (int ks = 0; ks < D / 32; ++ks) kr[kt][ks] = load16(base + off + 32 * ks);
+        for (int ks = 0; ks < D / 32; ++ks) kr[kt][ks] = load16_at(base + 32 * ks, off);
       }
     };
-    int b = tiles > 0 ? next_block(wk + KW * split - step) : n_blocks;
-    if (b < n_blocks) load_keys(b);
-    while (b < n_blocks) {
+    if (rest) load_keys(__builtin_ctz(rest));
+    while (rest) {
+      const int b = __builtin_ctz(rest);
       const bool ring = b < RB;
       {
         const uint16_t* base = ring ? ro.ring_v + b * (KB * D) : ro.v + (int64_t)(b - RB) * KB * p.nv_sl;
@@ -413,11 +433,12 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
         const int last = ring ? KB - 1 : len - 1 - (b - RB) * KB;
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
-          const uint32_t off = (uint32_t)min(16 * (s >> 2) + 4 * g4 + (s & 3), last) * st + 8 * c;
-          vr[0][s] = load16(base + off);
-          vr[1][s] = load16(base + off + 128);
+          const uint32_t off = 2 * ((uint32_t)min(16 * (s >> 2) + 4 * g4 + (s & 3), last) * st + 8 * c);
+          vr[0][s] = load16_at(base, off);
+          vr[1][s] = load16_at(base + 128, off);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);   // the loads are issued here, before the scores wait for the keys
       f32x4 S[T][2];
 #pragma unroll
       for (int t = 0; t < T; ++t) S[t][0] = S[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -429,11 +450,11 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
           S[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[0][ks]), qf, S[t][0], 0, 0, 0);
           S[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[1][ks]), qf, S[t][1], 0, 0, 0);
         }
-      const int b_now = b;
-      b = next_block(b);
-      if (b < n_blocks) load_keys(b);
+      rest &= rest - 1;
+      if (rest) load_keys(__builtin_ctz(rest));
+      __builtin_amdgcn_sched_barrier(0);
       bf16x8 pb[T];
-      softmax(b_now, S, pb);
+      softmax(b, S, pb);
       add_values(0, vr[0], pb);
       add_values(1, vr[1], pb);
     }
@@ -444,34 +465,47 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
       const bool ring = b < RB;
       const uint16_t* kb = ring ? ro.ring_k + b * (KB * D) : ro.k + (int64_t)(b - RB) * KB * p.nk_sl;
       const uint16_t* vb = ring ? ro.ring_v + b * (KB * D) : ro.v + (int64_t)(b - RB) * KB * p.nv_sl;
-      const uint32_t k_st = ring ? D : (uint32_t)p.nk_sl, v_st = ring ? D : (uint32_t)p.nv_sl;
-      const int last = ring ? KB - 1 : len - 1 - (b - RB) * KB;
-      const uint32_t to = lds_offset(&lds.stage[stage]);
+      const uint32_t to = lds_offset(&lds.stage[stage]) + 1024 * (EACH / 2) * wave;
+      // load e of the wave brings rows 2 o and 2 o + 1 of keys and values, o = wave * (EACH / 2) + e
+      const int l = lane_per_site(lane);
+      const int row = wave * EACH + (l >> 5);
+      const uint32_t k_piece = 16 * ((l & 31) ^ (row & 15)), v_piece = 16 * (l & 31);
 #pragma unroll
       for (int e = 0; e < EACH / 2; ++e) {
-        const int o = wave * (EACH / 2) + e;              // (key tile, k step) of the keys; two rows of the values
-        const uint32_t k_off = (uint32_t)min(16 * (o >> 3) + c, last) * k_st + 32 * (o & 7) + 8 * g4;
-        load_lds16(kb, 2 * k_off, __builtin_amdgcn_readfirstlane(to + 1024 * o));
-        const uint32_t v_off = (uint32_t)min(2 * o + (lane >> 5), last) * v_st + 8 * (lane & 31);
-        load_lds16(vb, 2 * v_off, __builtin_amdgcn_readfirstlane(to + (uint32_t)offsetof(KeyStage, v) + 1024 * o));
+        uint32_t k_off, v_off;
+        if (ring) {   // (row + 2 e: the rows of a wave share all but bits 1 and 2, which 2 e sets)
+          k_off = row * (2 * D) + (k_piece ^ (32 * e));
+          v_off = row * (2 * D) + v_piece;
+        } else {
+          const uint32_t at = (uint32_t)min(row + 2 * e, len - 1 - (b - RB) * KB);
+          k_off = at * (uint32_t)(2 * p.nk_sl) + (k_piece ^ (32 * e));
+          v_off = at * (uint32_t)(2 * p.nv_sl) + v_piece;
+        }
+        const int skip = ring ? 2 * e * D : 0;
+        load_lds16(kb + skip, k_off, to + 1024 * e);
+        load_lds16(vb + skip, v_off, to + (uint32_t)offsetof(KeyStage, v) + 1024 * e);
       }
     };
-    int b = next_block(split - step), stage = 0;
-    if (b < n_blocks) fetch(b, 0);
-    while (b < n_blocks) {
+    int stage = 0;
+    if (rest) fetch(__builtin_ctz(rest), 0);
+    while (rest) {
+      const int b = __builtin_ctz(rest);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // the block has landed
       __builtin_amdgcn_s_barrier();                       // for every wave; and the block before is read no more
       asm volatile("" ::: "memory");
-      const int b_next = next_block(b);
-      if (b_next < n_blocks) fetch(b_next, stage ^ 1);
+      rest &= rest - 1;
+      if (rest) fetch(__builtin_ctz(rest), stage ^ 1);
       if (tiles > 0) {
         const KeyStage& ks_ = lds.stage[stage];
+        const int c_here = lane_per_site(c);   // the addresses are made here rather than kept over the loop
         f32x4 S[T][2];
 #pragma unroll
         for (int t = 0; t < T; ++t) S[t][0] = S[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < D / 32; ++ks) {
-          const bf16x8 k0 = as_bf16x8(ks_.k[0][ks][lane]), k1 = as_bf16x8(ks_.k[1][ks][lane]);
+          // pieces 4 ks + g4 and 16 more share an address: the permutation takes the low 4 bits
+          const uint16_t* const at = &ks_.k[c][8 * ((4 * (ks & 3) + g4) ^ c_here) + 128 * (ks >> 2)];
+          const bf16x8 k0 = as_bf16x8(load16(at)), k1 = as_bf16x8(load16(at + 16 * D));
 #pragma unroll
           for (int t = 0; t < T; ++t) {
             S[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qr[t][ks], S[t][0], 0, 0, 0);
@@ -489,49 +523,65 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
           add_values(hh, vr, pb);
         }
       }
-      b = b_next;
       stage ^= 1;
     }
   }
 
   // ---- the waves' partial sums meet; outputs ----
+  // (rows and addresses are made again here rather than kept over the loop)
+  const int lane_end = lane_per_site(lane);
+  const int ge = lane_end >> 4, ce = lane_end & 15;
+  // lane (ge, ce) of product (hh, i), register r: query ce, dim 128 hh + 32 ge + 8 r + i; a lane stores 8 R dims at a time
+  constexpr int R = KW > 1 ? 8 / KW : 4;
+  constexpr int TIMES = KW > 1 ? 1 : 2;
+  const auto half_of = [&](int x) { return KW > 1 ? wk * R / 4 : x; };
+  const int r0 = KW > 1 ? wk * R % 4 : 0;
+  // gates are loaded before the outputs that they could alias are stored: all of them, or (STAGED: registers) a tile's
+  u32x4 gw[STAGED ? 1 : T][TIMES][R];
+  const auto load_gates = [&](int t, int to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < TIMES; ++x)
+      load_gate(p, ro, min(r_lo + 16 * t + ce, M - 1), 128 * half_of(x) + 32 * ge + 8 * r0, gw[to][x]);
+  };
+  if (!STAGED && p.splits == 1) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) load_gates(t, t);
+  }
 #pragma unroll
   for (int t = 0; t < T; ++t) sum[t] = add_xor32(add_xor16(sum[t]));
   if constexpr (KW > 1) {
 #pragma unroll
     for (int t = 0; t < T; ++t)
-      if (g4 == 0) {
-        lds.ml[wave][t][c][0] = m[t];
-        lds.ml[wave][t][c][1] = sum[t];
+      if (ge == 0) {
+        lds.ml[wave][t][ce][0] = m[t];
+        lds.ml[wave][t][ce][1] = sum[t];
       }
     __syncthreads();   // (the queries in LDS are read no more, either)
   }
-  // lane (g4, c) of product (hh, i), register r: query c, dim 128 hh + 32 g4 + 8 r + i; a lane stores 8 R dims at a time
-  constexpr int R = KW > 1 ? 8 / KW : 4;
-  constexpr int TIMES = KW > 1 ? 1 : 2;
 #pragma unroll
   for (int t = 0; t < T; ++t) {
-    const int row = r_lo + 16 * t + c;
+    const int row = r_lo + 16 * t + ce;
+    if (STAGED && p.splits == 1) load_gates(t, 0);
     float top = m[t], total = sum[t];
     if constexpr (KW > 1) {
       top = -INFINITY;
       total = 0.f;
 #pragma unroll
-      for (int w = 0; w < KW; ++w) top = fmaxf(top, lds.ml[wq * KW + w][t][c][0]);
+      for (int w = 0; w < KW; ++w) top = fmaxf(top, lds.ml[wq * KW + w][t][ce][0]);
       const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-      for (int w = 0; w < KW; ++w) total += exp2_fast(lds.ml[wq * KW + w][t][c][0] - base) * lds.ml[wq * KW + w][t][c][1];
+      for (int w = 0; w < KW; ++w) total += exp2_fast(lds.ml[wq * KW + w][t][ce][0] - base) * lds.ml[wq * KW + w][t][ce][1];
       const float mine = exp2_fast(m[t] - base);
       if (t) __syncthreads();   // the tile before is read
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) lds.o[wave][8 * hh + i][lane] = O[t][hh][i] * mine;
+        for (int i = 0; i < 8; ++i) lds.o[wave][8 * hh + i][lane_end] = O[t][hh][i] * mine;
       __syncthreads();
     }
 #pragma unroll
     for (int x = 0; x < TIMES; ++x) {
-      const int hh = KW > 1 ? wk * R / 4 : x, r0 = KW > 1 ? wk * R % 4 : 0;
+      const int hh = half_of(x);
       float y[8 * R];
       if constexpr (KW > 1) {
 #pragma unroll
@@ -540,7 +590,7 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
         for (int w = 0; w < KW; ++w)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float* src = reinterpret_cast<const float*>(&lds.o[wq * KW + w][8 * hh + i][lane]) + r0;
+            const float* src = reinterpret_cast<const float*>(&lds.o[wq * KW + w][8 * hh + i][lane_end]) + r0;
 #pragma unroll
             for (int r = 0; r < R; ++r) y[8 * r + i] += src[r];
           }
@@ -550,20 +600,20 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
 #pragma unroll
           for (int r = 0; r < 4; ++r) y[8 * r + i] = O[t][x][i][r];
       }
-      const int d0 = 128 * hh + 32 * g4 + 8 * r0;
+      const int d0 = 128 * hh + 32 * ge + 8 * r0;
       if (row >= M) continue;
       if (p.splits == 1) {
         const float inv = 1.0f / total;
 #pragma unroll
         for (int e = 0; e < 8 * R; ++e) y[e] *= inv;
-        if (!all_finite(y)) atomicOr(&lds.odd[wq * T + t], 1u << c);
-        store_gated(p, ro, row, d0, y);
+        if (!all_finite(y)) atomicOr(&lds.odd[wq * T + t], 1u << ce);
+        store_gated(p, ro, row, d0, y, gw[STAGED ? 0 : t][x]);
       } else {
         const int64_t at = ((int64_t)pair * p.splits + split) * ((int64_t)G * p.max_nodes) + row;
         float* dst = p.part_o + at * D + d0;
 #pragma unroll
         for (int e = 0; e < 8 * R; e += 4) *reinterpret_cast<f32x4*>(dst + e) = (f32x4){y[e], y[e + 1], y[e + 2], y[e + 3]};
-        if (hh == 0 && g4 == 0 && r0 == 0) {
+        if (hh == 0 && ge == 0 && r0 == 0) {
           p.part_ml[2 * at] = top;
           p.part_ml[2 * at + 1] = total;
         }
@@ -575,44 +625,64 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
   __syncthreads();   // also: the stores of these rows' first results are done
   for (int i = threadIdx.x >> 5; i < ROWS; i += 64 * NW / 32)
     if (lds.odd[i >> 4] >> (i & 15) & 1u) {
+      const int d0 = 8 * (threadIdx.x & 31);
       float y[8];
-      walk_keys(p, ro, r_wg + i, 8 * (threadIdx.x & 31), y);
-      store_gated(p, ro, r_wg + i, 8 * (threadIdx.x & 31), y);
+      u32x4 one[1];
+      load_gate(p, ro, r_wg + i, d0, one);
+      walk_keys(p, ro, r_wg + i, d0, y);
+      store_gated(p, ro, r_wg + i, d0, y, one);
     }
 }
 
-// Joins the splits' partial sums: 16 lanes a query row, 16 dims a lane
+// Joins the splits' partial sums: a wave a query row, 4 dims a lane; every split's loads are in flight at once
+constexpr int SPLITS_MAX = 8;
 __global__ __launch_bounds__(256) void tree_attn_join_kernel(const TreeAttnParams p) {
   const int pair = blockIdx.x;
   const int n = pair / p.hkv, h = pair - n * p.hkv;
-  TreeKeys ro;
-  if (!tree_keys(p, n, h, ro)) return;
-  const int row = blockIdx.y * 16 + (threadIdx.x >> 4), d0 = 16 * (threadIdx.x & 15);
-  if (row >= p.G * ro.len) return;
+  const int row = blockIdx.y * 4 + (threadIdx.x >> 6), d0 = 4 * (threadIdx.x & 63);
   const int64_t stride = (int64_t)p.G * p.max_nodes;
   const int64_t first = (int64_t)pair * p.splits * stride + row;
+  f32x4 v[SPLITS_MAX];
+  float m[SPLITS_MAX], l[SPLITS_MAX];
+  if (row >= stride) return;
+#pragma unroll
+  for (int s = 0; s < SPLITS_MAX; ++s) {
+    const int64_t at = first + min(s, p.splits - 1) * stride;   // (a row of no tree: whatever the workspace holds, not used)
+    v[s] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + d0);
+    m[s] = p.part_ml[2 * at];
+    l[s] = p.part_ml[2 * at + 1];
+  }
+  TreeKeys ro;
+  if (!tree_keys(p, n, h, ro) || row >= p.G * ro.len) return;
+  const int node = row / p.G, g = row - node * p.G;
+  u32x2 gate = {0u, 0u};
+  if (ro.gate) gate = *reinterpret_cast<const u32x2*>(ro.gate + node * p.g_sl + g * p.g_sg + d0);
   float top = -INFINITY, total = 0.f;
-  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[2 * (first + s * stride)]);
+#pragma unroll
+  for (int s = 0; s < SPLITS_MAX; ++s)
+    if (s < p.splits) top = fmaxf(top, m[s]);
   const float base = top == -INFINITY ? 0.f : top;
-  float y[16];
+  float y[4] = {};
 #pragma unroll
-  for (int e = 0; e < 16; ++e) y[e] = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float w = exp2_fast(p.part_ml[2 * (first + s * stride)] - base);
-    total += w * p.part_ml[2 * (first + s * stride) + 1];
-    const float* src = p.part_o + (first + s * stride) * D + d0;
+  for (int s = 0; s < SPLITS_MAX; ++s) {
+    if (s >= p.splits) continue;
+    const float w = exp2_fast(m[s] - base);
+    total = __builtin_fmaf(w, l[s], total);
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(src + e);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[e + i] = __builtin_fmaf(w, v[i], y[e + i]);
-    }
+    for (int i = 0; i < 4; ++i) y[i] = __builtin_fmaf(w, v[s][i], y[i]);
   }
   const float inv = 1.0f / total;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) y[e] *= inv;
+  for (int e = 0; e < 4; ++e) y[e] *= inv;
   if (!all_finite(y)) walk_keys(p, ro, row, d0, y);
-  store_gated(p, ro, row, d0, y);
+  if (ro.gate) {
+    float gt[4];
+    unpack2(gate[0], gt[0], gt[1]);
+    unpack2(gate[1], gt[2], gt[3]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] *= sigmoidf_(gt[e]);
+  }
+  store4_bf16(ro.out + node * p.o_sl + g * p.o_sg + d0, y);
 }
 
 // The committed chain's keys and values into the ring (of a chain longer than the window its last W), 16 nodes a workgroup:
@@ -652,7 +722,7 @@ inline int rows_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : ro
 // of GB/s. 8 at most.
 inline int splits_of(int64_t n_rows, int64_t hkv, int64_t rows) {
   const int64_t units = n_rows * hkv * ((rows + rows_of(rows) - 1) / rows_of(rows));
-  return units <= 32 ? 8 : units <= 64 ? 4 : units <= 128 ? 2 : 1;
+  return units <= 32 ? SPLITS_MAX : units <= 64 ? 4 : units <= 128 ? 2 : 1;
 }
 
 inline size_t part_bytes(int64_t n_rows, int64_t hkv, int64_t rows, int splits) {
@@ -724,7 +794,7 @@ extern "C" int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int
   else if (per_wg == 64) launch(tree_attn_kernel<2, 2, false>);
   else launch(tree_attn_kernel<2, 1, true>);
   if (p.splits > 1)
-    hipLaunchKernelGGL(tree_attn_join_kernel, dim3((unsigned)pairs, (unsigned)((rows + 15) / 16)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(tree_attn_join_kernel, dim3((unsigned)pairs, (unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
   if (commits)
     hipLaunchKernelGGL(tree_ring_write_kernel, dim3((unsigned)pairs, (unsigned)((max_nodes + 15) / 16)), dim3(256), 0, st, p);
   return launch_status();
