@@ -100,6 +100,12 @@ __device__ __forceinline__ u32x4 load16(const uint16_t* p) { return *reinterpret
 __device__ __forceinline__ u32x4 load16_at(const uint16_t* base, uint32_t off) {
   return *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + off);
 }
+// the largest of three, a NaN aside, in one instruction (fmaxf quiets its operands first, an instruction each)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // node i's ancestors and itself
@@ -360,16 +366,16 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
       }
     }
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-      top[t] = fmaxf(fmaxf(fmaxf(S[t][0][0], S[t][0][1]), fmaxf(S[t][0][2], S[t][0][3])),
-                     fmaxf(fmaxf(S[t][1][0], S[t][1][1]), fmaxf(S[t][1][2], S[t][1][3])));
-      top[t] = max_pair32(max_pair16(top[t])) * sl2;
+    for (int t = 0; t < T; ++t) {   // the lane's own keys tell whether the maximum moves
+      top[t] = max3(max3(S[t][0][0], S[t][0][1], S[t][0][2]), max3(S[t][0][3], S[t][1][0], S[t][1][1]),
+                    max3(S[t][1][2], S[t][1][3], -INFINITY)) * sl2;
       move |= top[t] > m[t] + SLACK;
     }
     if (__any(move)) {
 #pragma unroll
       for (int t = 0; t < T; ++t) {
-        const float to = top[t] > m[t] + SLACK ? top[t] : m[t];
+        const float high = max_pair32(max_pair16(top[t]));
+        const float to = high > m[t] + SLACK ? high : m[t];
         const float alpha = to == -INFINITY ? 1.f : exp2_fast(m[t] - to);
         m[t] = to;
         sum[t] *= alpha;
@@ -470,20 +476,21 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
       const int l = lane_per_site(lane);
       const int row = wave * EACH + (l >> 5);
       const uint32_t k_piece = 16 * ((l & 31) ^ (row & 15)), v_piece = 16 * (l & 31);
+      // (the rows of a wave share all but bits 1 and 2, which 2 e sets)
+      if (ring) {
+        const uint32_t k_off = row * (2 * D) + k_piece, v_off = row * (2 * D) + v_piece;
 #pragma unroll
-      for (int e = 0; e < EACH / 2; ++e) {
-        uint32_t k_off, v_off;
-        if (ring) {   // (row + 2 e: the rows of a wave share all but bits 1 and 2, which 2 e sets)
-          k_off = row * (2 * D) + (k_piece ^ (32 * e));
-          v_off = row * (2 * D) + v_piece;
-        } else {
-          const uint32_t at = (uint32_t)min(row + 2 * e, len - 1 - (b - RB) * KB);
-          k_off = at * (uint32_t)(2 * p.nk_sl) + (k_piece ^ (32 * e));
-          v_off = at * (uint32_t)(2 * p.nv_sl) + v_piece;
+        for (int e = 0; e < EACH / 2; ++e) {
+          load_lds16(kb + 2 * e * D, k_off ^ (32 * e), to + 1024 * e);
+          load_lds16(vb + 2 * e * D, v_off, to + (uint32_t)offsetof(KeyStage, v) + 1024 * e);
         }
-        const int skip = ring ? 2 * e * D : 0;
-        load_lds16(kb + skip, k_off, to + 1024 * e);
-        load_lds16(vb + skip, v_off, to + (uint32_t)offsetof(KeyStage, v) + 1024 * e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < EACH / 2; ++e) {
+          const uint32_t at = (uint32_t)min(row + 2 * e, len - 1 - (b - RB) * KB);
+          load_lds16(kb, at * (uint32_t)(2 * p.nk_sl) + (k_piece ^ (32 * e)), to + 1024 * e);
+          load_lds16(vb, at * (uint32_t)(2 * p.nv_sl) + v_piece, to + (uint32_t)offsetof(KeyStage, v) + 1024 * e);
+        }
       }
     };
     int stage = 0;
