@@ -723,7 +723,7 @@ __global__ __launch_bounds__(256) void tree_ring_write_kernel(const TreeAttnPara
 }
 
 // Query rows of a workgroup: from 65 on every wave has its own and the keys pass through LDS
-inline int rows_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+inline int rows_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 64 ? 64 : 128; }
 
 // Workgroups of a row's key blocks: few rows leave the chip (256 CUs) short of workgroups, and one CU moves only a few tens
 // of GB/s. 8 at most.
@@ -797,8 +797,7 @@ extern "C" int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NW), 0, st, p); };
   if (per_wg == 16) launch(tree_attn_kernel<1, 4, false>);
-  else if (per_wg == 32) launch(tree_attn_kernel<2, 4, false>);
-  else if (per_wg == 64) launch(tree_attn_kernel<2, 2, false>);
+  else if (per_wg == 64) launch(tree_attn_kernel<1, 1, true>);
   else launch(tree_attn_kernel<2, 1, true>);
   if (p.splits > 1)
     hipLaunchKernelGGL(tree_attn_join_kernel, dim3((unsigned)pairs, (unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
