@@ -114,24 +114,35 @@ __global__ __launch_bounds__(256) void tree_conv_kernel(const uint16_t* x, int64
   const int c = blockIdx.x * CH + 8 * col;
   const bool mine = c < channels;
   uint16_t* const hist = pool + slot * (TAPS - 1) * channels + c;
-  u32x4 piece[EACH];
+  // every load is in flight before the first is waited for
+  constexpr int OLD = (TAPS - 1 + STEP - 1) / STEP;   // history rows of a thread
+  u32x4 piece[EACH], old[OLD], wt[TAPS] = {};
+  uint64_t mask[EACH];
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
     const int i = first + STEP * e;
-    if (mine && i < len) piece[e] = *reinterpret_cast<const u32x4*>(x + (off + i) * x_stride + c);
+    if (i >= len || !mine) break;
+    piece[e] = *reinterpret_cast<const u32x4*>(x + (off + i) * x_stride + c);
+    mask[e] = (uint64_t)masks[off + i];
   }
-  u32x4 wt[TAPS] = {};
+#pragma unroll
+  for (int h = 0; h < OLD; ++h)
+    if (mine && first + STEP * h < TAPS - 1)
+      old[h] = *reinterpret_cast<const u32x4*>(hist + (int64_t)(first + STEP * h) * channels);
   if (mine && first < len) {
 #pragma unroll
     for (int t = 0; t < TAPS; ++t) wt[t] = *reinterpret_cast<const u32x4*>(weight + (int64_t)c * TAPS + 8 * t);
   }
-  for (int h = first; h < TAPS - 1; h += STEP)
-    if (mine) *reinterpret_cast<u32x4*>(&tile[(NODES + h) * CH + 8 * col]) = *reinterpret_cast<const u32x4*>(hist + (int64_t)h * channels);
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
     const int i = first + STEP * e;
-    if (mine && i < len) *reinterpret_cast<u32x4*>(&tile[i * CH + 8 * col]) = piece[e];
+    if (i >= len || !mine) break;
+    *reinterpret_cast<u32x4*>(&tile[i * CH + 8 * col]) = piece[e];
   }
+#pragma unroll
+  for (int h = 0; h < OLD; ++h)
+    if (mine && first + STEP * h < TAPS - 1)
+      *reinterpret_cast<u32x4*>(&tile[(NODES + first + STEP * h) * CH + 8 * col]) = old[h];
   __syncthreads();
   if (!mine) return;
   // weight[channel][tap]: piece t holds channels 2 t and 2 t + 1
@@ -147,7 +158,7 @@ __global__ __launch_bounds__(256) void tree_conv_kernel(const uint16_t* x, int64
   for (int e = 0; e < EACH; ++e) {
     const int i = first + STEP * e;
     if (i >= len) break;
-    uint64_t up = (uint64_t)masks[off + i] & ((1ull << i) - 1);   // the ancestors not yet taken
+    uint64_t up = mask[e] & ((1ull << i) - 1);                    // the ancestors not yet taken
     int row[TAPS];
     row[0] = i;
     int h = TAPS - 1;                                             // the next history row up, plus one
