@@ -26,7 +26,8 @@ import numpy as np
 import torch
 
 from .. import _hostpack
-from .._lib import HSG_ERR_SHAPE, HSG_GDN_BURST_MIN_DEFAULT, HSG_GEMM_SKINNY_M_MAX, calls, check, lib
+from .._lib import (HSG_ERR_SHAPE, HSG_GDN_BURST_MIN_DEFAULT, HSG_GEMM_SKINNY_M_MAX, HSG_TREE_MAX_NODES, calls, check,
+                    lib)
 from ..model import ROLES, GuardModel
 from .gemm_plan import WORKSPACE_BYTES as GEMM_WORKSPACE_BYTES
 from .gemm_plan import GemmPlans
@@ -37,6 +38,8 @@ STATE_DTYPES = {"float32": torch.float32, "float16": torch.float16}
 _STATE_CODE = {torch.float32: 0, torch.float16: 1}
 # Tokens of a long piece (SlotStreamEngine._run_long): enough for the products to run at their large-M rate
 LONG_TOKENS = 4096
+# Bounds on the nodes of a drafted tree by which tree ticks are captured: the tree kernels' tiles follow them
+TREE_BUCKETS = (4, 16, 32, HSG_TREE_MAX_NODES)
 
 
 def bucket(value, choices):
@@ -90,6 +93,26 @@ def pack_ticks(chunks, slots, length, nb, tb, max_slots, out):
     sts[:n] = starts
     sts[n:] = 0
     return lens, offsets
+
+
+def pack_trees(trees, slots, length, nb, tb, max_slots, out):
+    """Packed layout of a tick of drafted trees, (ids, parents, commits) each, in one int64 buffer ``[ids tb | parents tb |
+    lens nb | slots nb | starts nb | commits nb]``; rows n >= len(trees) are padding (no nodes, the scratch slot), tokens
+    past the real ones carry id 0. The device builds offsets, positions and ancestors from it (hsg_tree_maps). Returns
+    (lens [n], offsets [n])."""
+    n = len(trees)
+    lens = np.fromiter((len(t[0]) for t in trees), dtype=np.int64, count=n)
+    total = int(lens.sum())
+    out[:] = 0
+    for at, which in ((0, 0), (tb, 1)):
+        out[at:at + total] = np.fromiter(itertools.chain.from_iterable(t[which] for t in trees), dtype=np.int64,
+                                         count=total)
+    rows = out[2 * tb:].reshape(4, nb)
+    rows[0, :n] = lens
+    rows[1, :n], rows[1, n:] = slots, max_slots
+    rows[2, :n] = np.asarray(length, dtype=np.int64)[slots]
+    rows[3, :n] = [t[2] for t in trees]
+    return lens, np.cumsum(lens) - lens
 
 
 def gdn_proj_width(cfg):
@@ -399,11 +422,31 @@ class SlotStreamEngine(PreparedWeights):
                 "lens": x[2 * tb + nb:2 * tb + 2 * nb], "slots": x[2 * tb + 2 * nb:2 * tb + 3 * nb],
                 "starts": x[2 * tb + 3 * nb:2 * tb + 4 * nb], "all": x[:2 * tb + 4 * nb]}
 
-    def _forward(self, nb, tb, inp, scratch=None, max_len=0, short_rows=True):
+    def _tree_inputs(self, nb, tb):
+        x = self.buf["inputs"]
+        rows = x[2 * tb:2 * tb + 4 * nb].view(4, nb)
+        return {"ids": x[:tb], "parents": x[tb:2 * tb], "lens": rows[0], "slots": rows[1], "starts": rows[2],
+                "commits": rows[3], "all": x[:2 * tb + 4 * nb]}
+
+    def _tree_buffers(self):
+        """The maps and the attention workspace of a tick of trees, once for every shape of it: the captured graphs hold
+        their addresses."""
+        if not hasattr(self, "tree_maps"):
+            cfg = self.cfg
+            hkv = cfg.num_key_value_heads
+            need = max(lib().hsg_tree_attention_workspace_bytes(rows, hkv, cfg.num_attention_heads // hkv, cap)
+                       for rows in self.session_buckets for cap in TREE_BUCKETS)
+            self.tree_maps = torch.zeros(2 * self.max_tokens + 3 * self.max_rows, dtype=torch.long, device=self.device)
+            self.tree_ws = torch.empty(max(int(need), 16), dtype=torch.uint8, device=self.device)
+        return self.tree_maps, self.tree_ws
+
+    def _forward(self, nb, tb, inp, scratch=None, max_len=0, short_rows=True, tree=None):
         """The tick's device program (src/hs_guard/engine/slot_engine_v8.py:30-58), launched on the current
         stream. Reads only device memory, so it can be captured into a hipGraph. max_len > 0: a long piece's program
         (_run_long) over its own ``scratch``, every row of up to max_len tokens on hsg_ring_prefill and, from
-        chunk_min_tokens on, the chunk kernels (short_rows False: no row is shorter)."""
+        chunk_min_tokens on, the chunk kernels (short_rows False: no row is shorter). tree (most nodes of a row, whether
+        rows may commit): a tick of drafted trees (step_tree), whose mixers are the tree kernels and leave every pool as it
+        is but for the committed chains."""
         L = calls()
         long = max_len > 0
         buf, chunk_ws = scratch or (self.buf, getattr(self, "chunk_ws", None))
@@ -420,8 +463,20 @@ class SlotStreamEngine(PreparedWeights):
         G = hq // hkv
         nh, hv, kd, vd = cfg.linear_num_key_heads, cfg.linear_num_value_heads, cfg.linear_key_head_dim, \
             cfg.linear_value_head_dim
-        ids, pos, offsets, lens, slots, starts = (inp[k] for k in ("ids", "pos", "offsets", "lens", "slots",
-                                                                    "starts"))
+        if tree:
+            nodes, moves = tree
+            maps, tree_ws = self._tree_buffers()
+            pos, masks = maps[:tb], maps[tb:2 * tb]
+            offsets, lens, commits = (maps[2 * tb + i * nb:2 * tb + (i + 1) * nb] for i in range(3))
+            ids, slots, starts = inp["ids"], inp["slots"], inp["starts"]
+            check(L.hsg_tree_maps(inp["parents"].data_ptr(), tb, inp["lens"].data_ptr(), starts.data_ptr(),
+                                  inp["commits"].data_ptr(), nb, nodes, offsets.data_ptr(), lens.data_ptr(),
+                                  commits.data_ptr(), pos.data_ptr(), masks.data_ptr(), st), "hsg_tree_maps")
+            tree_rows = (lens.data_ptr(), offsets.data_ptr(), commits.data_ptr() if moves else None, masks.data_ptr(), nb,
+                         nodes)
+        else:
+            ids, pos, offsets, lens, slots, starts = (inp[k] for k in ("ids", "pos", "offsets", "lens", "slots",
+                                                                        "starts"))
         hid = [view("hidden", tb, H)]
         normed = view("normed", tb, H)
         mix = view("mix", tb, H)
@@ -462,7 +517,18 @@ class SlotStreamEngine(PreparedWeights):
                 # rows are packed longest first: in a prefill-like tick the rows of >= chunk_min_tokens tokens go
                 # to the chunked kernels (one WY/UT chunk each), the rest to the slot step
                 R = nb if long else self._chunk_rows(nb, tb)
-                if self.fuse_conv and R == 0:
+                if tree:
+                    conv = view("conv", tb, C)
+                    check(L.hsg_tree_conv_silu(base, self.gdn_in, self.conv[idx].data_ptr(), S, Lw["conv_w"].data_ptr(),
+                                               cfg.linear_conv_kernel_dim, slots.data_ptr(), *tree_rows, C, conv.data_ptr(),
+                                               C, st), "hsg_tree_conv_silu")
+                    check(L.hsg_gdn_tree_step(
+                        conv.data_ptr(), C, 0, cfg.key_dim, 2 * cfg.key_dim, base + 2 * (C + cfg.value_dim + hv),
+                        base + 2 * (C + cfg.value_dim), self.gdn_in, Lw["A_log"].data_ptr(), Lw["dt_bias"].data_ptr(),
+                        self.rec[idx].data_ptr(), _STATE_CODE[self.state_dtype], S, slots.data_ptr(), *tree_rows, nh, hv,
+                        kd, vd, kd ** -0.5, base + 2 * C, self.gdn_in, Lw["norm_w"].data_ptr(), eps, out.data_ptr(), st),
+                        "hsg_gdn_tree_step")
+                elif self.fuse_conv and R == 0:
                     # causal conv + SiLU inside the slot step, from the raw projection and the conv history pool
                     check(L.hsg_gdn_conv_slot_step_gated(
                         base, self.gdn_in, 0, cfg.key_dim, 2 * cfg.key_dim, Lw["conv_w"].data_ptr(),
@@ -507,7 +573,7 @@ class SlotStreamEngine(PreparedWeights):
                 k = view("k", tb, hkv * D)
                 base = proj.data_ptr()
                 att = view("mid", tb, hq * D)
-                if tb == 1 and cfg.rotary_dim == 64 and D == 256:
+                if tb == 1 and cfg.rotary_dim == 64 and D == 256 and not tree:
                     # a one-token tick: the q / k norm and RoPE run inside the decode's scores kernel (one launch
                     # fewer), bitwise hsg_norm_rope + hsg_ring_decode; k receives the new keys
                     check(L.hsg_ring_decode_rope(
@@ -526,7 +592,14 @@ class SlotStreamEngine(PreparedWeights):
                                           hq * D, D, base + 2 * hq * 2 * D, self.att_in, D, hkv,
                                           Lw["k_w1"].data_ptr(), eps, k.data_ptr(), hkv * D, D, pos.data_ptr(),
                                           self.inv_freq.data_ptr(), cfg.rotary_dim, tb, D, st), "hsg_norm_rope")
-                    if long:
+                    if tree:
+                        check(L.hsg_tree_attention(
+                            q.data_ptr(), hq * D, G * D, D, self.ring_k[idx].data_ptr(), self.ring_v[idx].data_ptr(), S, W,
+                            k.data_ptr(), hkv * D, D, base + 2 * (hq * 2 * D + hkv * D), self.att_in, D,
+                            base, self.att_in, G * 2 * D, 2 * D, D, self.ring_pos.data_ptr(), slots.data_ptr(),
+                            starts.data_ptr(), *tree_rows, hkv, G, D, D ** -0.5, att.data_ptr(), hq * D, G * D, D,
+                            tree_ws.data_ptr(), tree_ws.numel(), st), "hsg_tree_attention")
+                    elif long:
                         check(L.hsg_ring_prefill(
                             q.data_ptr(), hq * D, G * D, D, self.ring_k[idx].data_ptr(), self.ring_v[idx].data_ptr(), S,
                             W, k.data_ptr(), hkv * D, D, base + 2 * (hq * 2 * D + hkv * D), self.att_in, D,
@@ -583,8 +656,10 @@ class SlotStreamEngine(PreparedWeights):
         check(L.hsg_risk_head(y.data_ptr(), R * E, self.head_ln_w.data_ptr(), self.head_ln_b.data_ptr(),
                               self.head_w2.data_ptr(), self.head_b2.data_ptr(), cfg.layer_norm_eps, R, E,
                               probs.data_ptr(), tb, st), "hsg_risk_head")
-        check(L.hsg_ring_pos_update(self.ring_pos.data_ptr(), S, W, slots.data_ptr(), starts.data_ptr(),
-                                    lens.data_ptr(), nb, max_len or self.max_tick_tokens, st), "hsg_ring_pos_update")
+        if not tree or moves:
+            moved = commits if tree else lens
+            check(L.hsg_ring_pos_update(self.ring_pos.data_ptr(), S, W, slots.data_ptr(), starts.data_ptr(),
+                                        moved.data_ptr(), nb, max_len or self.max_tick_tokens, st), "hsg_ring_pos_update")
         return probs
 
     def _chunk_rows(self, nb, tb):
@@ -594,10 +669,10 @@ class SlotStreamEngine(PreparedWeights):
             return 0
         return nb
 
-    def _static(self, nb, tb):
-        key = (nb, tb)
+    def _static(self, nb, tb, tree=None):
+        key = (nb, tb, tree) if tree else (nb, tb)
         if key not in self.graphs:
-            inp = self._inputs(nb, tb)
+            inp = self._tree_inputs(nb, tb) if tree else self._inputs(nb, tb)
             inp["all"].zero_()
             inp["slots"].fill_(self.max_slots)       # empty rows on the scratch slot: no state is touched
             graph = None
@@ -606,11 +681,11 @@ class SlotStreamEngine(PreparedWeights):
                 side.wait_stream(torch.cuda.current_stream(self.device))
                 with torch.cuda.stream(side):
                     for _ in range(2):
-                        self._forward(nb, tb, inp)
+                        self._forward(nb, tb, inp, tree=tree)
                 torch.cuda.current_stream(self.device).wait_stream(side)
                 graph = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(graph, pool=self.pool):
-                    probs = self._forward(nb, tb, inp)
+                    probs = self._forward(nb, tb, inp, tree=tree)
                 self.pool = graph.pool()
                 self.stats["captures"] += 1
                 # the first replay of a graph pays a one-time upload; pay it here (inputs still address only
@@ -631,6 +706,13 @@ class SlotStreamEngine(PreparedWeights):
         nb = bucket(rows, self.session_buckets)
         for tb in sorted({bucket(t, self.token_buckets) for t in token_counts}):
             self._static(nb, tb)
+
+    @torch.inference_mode()
+    def prepare_trees(self, rows, token_counts, max_nodes, commits=False):
+        """``prepare`` for ticks of ``rows`` drafted trees of at most ``max_nodes`` nodes, that commit or do not."""
+        nb = bucket(rows, self.session_buckets)
+        for tb in sorted({bucket(t, self.token_buckets) for t in token_counts}):
+            self._static(nb, tb, (bucket(max_nodes, TREE_BUCKETS), bool(commits)))
 
     def _run_arrays(self, chunks, slots):
         """One tick: <= max_rows rows of <= max_tick_tokens tokens. Returns (probs [R, T, 3] numpy, lens,
@@ -715,7 +797,7 @@ class SlotStreamEngine(PreparedWeights):
                 # the reference's contract (docs/ENGINE.md:9): the embedding gather must never see an id it lacks
                 raise ValueError("Each request requires nonempty in-vocabulary integer token IDs")
 
-    def _replay(self, nb, tb, graph, inp, probs, host_in, host_out):
+    def _replay(self, nb, tb, graph, inp, probs, host_in, host_out, tree=None):
         """Send the packed inputs, run the tick (graph replay, or eagerly without graphs) and bring the
         probabilities back; returns when they are on the host."""
         inp["all"].copy_(host_in, non_blocking=True)
@@ -723,7 +805,7 @@ class SlotStreamEngine(PreparedWeights):
             graph.replay()
             self.stats["graph_replays"] += 1
         else:
-            probs = self._forward(nb, tb, inp)
+            probs = self._forward(nb, tb, inp, tree=tree)
             self.stats["eager_steps"] += 1
         host_out.copy_(probs, non_blocking=True)
         torch.cuda.current_stream(self.device).synchronize()
@@ -772,6 +854,73 @@ class SlotStreamEngine(PreparedWeights):
         flat, lens, offsets = self._run_arrays([c if isinstance(c, list) else list(c) for _, c in requests], slots)
         lb = bucket(int(lens.max()), (1, 2, 4, 8, 16, 32, 64))
         return padded_rows(flat, lens, offsets, lb), lens
+
+    def _check_trees(self, requests):
+        """step_tree's requests as (slot, ids, parents, commits), checked: what the device would reject raises here."""
+        out, seen, moving = [], set(), set()
+        for request in requests:
+            if len(request) not in (3, 4):
+                raise ValueError("A drafted tree is (slot, token_ids, parents) or (slot, token_ids, parents, commits)")
+            slot, ids, parents = request[:3]
+            commits = request[3] if len(request) == 4 else 0
+            if not isinstance(slot, (int, np.integer)) or not 0 <= slot < self.max_slots:
+                raise ValueError("Slot is outside the allocated range")
+            a, p = np.asarray(ids), np.asarray(parents)
+            if a.size == 0 or a.dtype.kind not in "iu" or a.ndim != 1 or int(a.min()) < 0 or int(a.max()) >= \
+                    self.cfg.vocab_size:
+                raise ValueError("Each request requires nonempty in-vocabulary integer token IDs")
+            if a.size > self.max_tick_tokens:
+                raise ValueError(f"A drafted tree has at most {self.max_tick_tokens} nodes")
+            index = np.arange(a.size)
+            if p.shape != a.shape or p.dtype.kind not in "iu" or (p < -1).any() or (p >= index).any():
+                raise ValueError("parents are one for each node, -1 or a node before it")
+            if not isinstance(commits, (int, np.integer)) or not 0 <= commits <= a.size or \
+                    (p[:commits] != index[:commits] - 1).any():
+                raise ValueError("commits counts leading nodes that are a chain from the session's last token")
+            if slot in moving or (commits and slot in seen):
+                raise ValueError("a session whose tree commits may appear once per tick")
+            seen.add(slot)
+            if commits:
+                moving.add(slot)
+            out.append((int(slot), a.tolist(), p.tolist(), int(commits)))
+        return out
+
+    def _run_trees(self, part):
+        """One tick of checked trees. Returns as _run_arrays."""
+        n = len(part)
+        row_lens = np.fromiter((len(ids) for _, ids, _, _ in part), dtype=np.int64, count=n)
+        total = int(row_lens.sum())
+        slots = np.fromiter((slot for slot, _, _, _ in part), dtype=np.int64, count=n)
+        commits = np.fromiter((c for _, _, _, c in part), dtype=np.int64, count=n)
+        nb, tb = bucket(n, self.session_buckets), bucket(total, self.token_buckets)
+        tree = (bucket(int(row_lens.max()), TREE_BUCKETS), bool(commits.any()))
+        graph, inp, probs, host_in, host_np, host_out, out_np = self._static(nb, tb, tree)
+        order = np.argsort(-row_lens, kind="stable")
+        lens_p, offsets_p = pack_trees([part[r][1:] for r in order], slots[order], self.length, nb, tb, self.max_slots,
+                                       host_np)
+        lens, offsets = np.empty(n, dtype=np.int64), np.empty(n, dtype=np.int64)
+        lens[order] = lens_p
+        offsets[order] = offsets_p
+        self._replay(nb, tb, graph, inp, probs, host_in, host_out, tree)
+        np.add.at(self.length, slots, commits)
+        return out_np[:, :total].copy(), lens, offsets
+
+    @torch.inference_mode()
+    def step_tree(self, requests):
+        """Scores drafted trees of live sessions without moving their state: requests (slot, token_ids, parents), parents[i]
+        the node that token i continues, a node before it, or -1 for the session's last token; at most max_tick_tokens
+        nodes. A fourth value ``commits`` accepts the tree's first nodes, a chain from the session's last token, which move
+        the session as step() would. A session may bring several trees to a call if none of them commits. Returns as
+        step(): {role: [CPU tensor [L_i, 3]]}, each node's class probabilities after its own path."""
+        trees = self._check_trees(requests)
+        results = {role: [] for role in self.roles}
+        for start in range(0, len(trees), self.max_rows):
+            flat, lens, offsets = self._run_trees(trees[start:start + self.max_rows])
+            probs = torch.from_numpy(request_order(flat, lens, offsets))
+            sizes = lens.tolist()
+            for r, role in enumerate(self.roles):
+                results[role] += torch.split(probs[r], sizes)
+        return results
 
     def one_tick(self, scan):
         """Whether requests whose ``_hostpack.scan`` result is ``scan`` (they passed its checks) fit one tick."""

@@ -157,6 +157,24 @@ class StreamingGuard:
             at += k
         return records
 
+    def step_tree(self, requests, role="assistant"):
+        """Cut scores of drafted continuations, without moving the conversations: requests (slot, token_ids, parents) or
+        (slot, token_ids, parents, commits), as the engine's step_tree takes them. Returns step()'s records, one per
+        request, with a score for each node of its tree."""
+        if role not in ("user", "assistant"):
+            raise ValueError("role must be user or assistant")
+        if not requests:
+            raise ValueError("Each tick requires nonempty requests and unique slots")
+        import torch
+        tau = self.metadata["thresholds"][role]
+        outputs = self.engine.step_tree(requests)[role]
+        cut = (1 - torch.cat(outputs)[:, 0]).tolist()
+        records, at = [], 0
+        for request, p in zip(requests, outputs):
+            records.append({"slot": request[0], "cut_scores": cut[at:at + len(p)], "threshold": tau})
+            at += len(p)
+        return records
+
 
 # ------------------------------------------------------------------------------------------------------------
 # Complete-message scoring

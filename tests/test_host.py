@@ -304,3 +304,16 @@ def test_long_piece_scratch_fits_its_piece():
     assert size([65], LONG_TOKENS) * 25 <= full
     assert size([900] * 3, 1344) < full and size([70, 3, 65, 1, 2000, 9], 1024) < full
     assert size([LONG_TOKENS // 4] * 4, 1024) >= 100 << 20
+
+
+def test_pack_trees_lays_out_rows_and_padding():
+    import numpy as np
+
+    from hs_guard.engine.slot_engine import pack_trees
+    out = np.full(2 * 8 + 4 * 4, 7, dtype=np.int64)
+    trees = [([11, 12, 13], [-1, 0, 0], 1), ([21, 22], [-1, -1], 0)]
+    lens, offsets = pack_trees(trees, np.array([2, 0]), np.array([5, 0, 9]), 4, 8, 3, out)
+    assert lens.tolist() == [3, 2] and offsets.tolist() == [0, 3]
+    assert out[:8].tolist() == [11, 12, 13, 21, 22, 0, 0, 0]
+    assert out[8:16].tolist() == [-1, 0, 0, -1, -1, 0, 0, 0]
+    assert out[16:].reshape(4, 4).tolist() == [[3, 2, 0, 0], [2, 0, 3, 3], [9, 5, 0, 0], [1, 0, 0, 0]]
