@@ -204,9 +204,8 @@ __device__ __forceinline__ void walk_row(const TreeStepParams& p, const TreeRow&
   }
 }
 
-// MOVES: rows may commit. Without, S0's registers are free as soon as it is split, and small trees keep three workgroups on a CU.
-template <int NT, bool HALF, bool GATED, bool MOVES>
-__global__ __launch_bounds__(64 * NW, NT == 1 && !MOVES ? 3 : 2) void gdn_tree_kernel(const TreeStepParams p) {
+template <int NT, bool HALF, bool GATED>
+__global__ __launch_bounds__(64 * NW, NT == 1 ? 4 : NT == 2 ? 3 : 2) void gdn_tree_kernel(const TreeStepParams p) {
   constexpr int PARTS = HALF ? 2 : 3;
   __shared__ TreeStepLds<NT> lds;
   const int lane = threadIdx.x & 63;
@@ -214,7 +213,7 @@ __global__ __launch_bounds__(64 * NW, NT == 1 && !MOVES ? 3 : 2) void gdn_tree_k
   const int g4 = lane >> 4, c = lane & 15;
   const int n = blockIdx.x / p.HV, hv = blockIdx.x - n * p.HV;
   const int64_t slot = p.slots[n], len64 = p.lens[n], off = p.offsets[n];
-  const int64_t done64 = MOVES ? p.commits[n] : 0;
+  const int64_t done64 = p.commits ? p.commits[n] : 0;
   if ((slot < 0) | (slot >= p.state_rows) | (len64 <= 0) | (len64 > p.max_nodes)) return;
   const int len = (int)len64;
   const int tiles = (len + 15) >> 4;
@@ -534,7 +533,7 @@ __global__ __launch_bounds__(64 * NW, NT == 1 && !MOVES ? 3 : 2) void gdn_tree_k
   }
 
   // ---- the committed chain moves the state: u scaled, split as the state was, times k^T read from LDS transposed ----
-  if (MOVES && ro.done > 0) {
+  if (ro.done > 0) {
     const float ec = lds.eG[ro.done - 1];
     constexpr int NP = (NT + 1) / 2;     // pairs of tiles: a product takes 32 nodes, the lane's own 4 of either tile
     bf16x8 up[NP][2][3];
@@ -555,17 +554,16 @@ __global__ __launch_bounds__(64 * NW, NT == 1 && !MOVES ? 3 : 2) void gdn_tree_k
 #pragma unroll
       for (int j = 0; j < 2; ++j) split8<3>(x[j], up[t2][j]);
     }
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
+    // state rows 32 s ..: accumulator row 4 g4 + r is state row 32 s + 8 g4 + 4 hh + r, operand row m = c is k's dim 32 s +
+    // 8 (c / 4) + 4 hh + c % 4, which transpose reads of 4-value vectors 8 dims apart give
+    const auto move = [&](int s, const auto& was) __attribute__((always_inline)) {
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
-        // accumulator row 4 g4 + r is state row 32 s + 8 g4 + 4 hh + r: operand row m = c is k's dim 32 s + 8 (c / 4) + 4 hh
-        // + c % 4, which transpose reads of 4-value vectors 8 dims apart give
         f32x4 acc[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[j][r] = ec * s0(s, j, 4 * hh + r);
+          for (int r = 0; r < 4; ++r) acc[j][r] = ec * was(j, 4 * hh + r);
 #pragma unroll
         for (int t2 = 0; t2 < NP; ++t2) {
           if (32 * t2 >= ro.done) break;
@@ -590,6 +588,30 @@ __global__ __launch_bounds__(64 * NW, NT == 1 && !MOVES ? 3 : 2) void gdn_tree_k
           else *reinterpret_cast<f32x2*>(at) = (f32x2){acc[0][r], acc[1][r]};
         }
       }
+    };
+    if constexpr (NT == 4) {   // LDS leaves two workgroups a CU, and them the registers to keep S0
+#pragma unroll
+      for (int s = 0; s < 4; ++s) move(s, [&](int j, int i) { return s0(s, j, i); });
+    } else {
+      // S0 again, from a cache, 32 rows at a time and the next ones on their way
+      const StatePair* const again = reinterpret_cast<const StatePair*>(state + lane_per_site(state_lane));
+      StatePair old[8], next[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) next[i] = again[i * (KD / 2)];
+#pragma unroll 1
+      for (int s = 0; s < 4; ++s) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) old[i] = next[i];
+        if (s < 3) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) next[i] = again[(32 * (s + 1) + i) * (KD / 2)];
+        }
+        move(s, [&](int j, int i) {
+          if constexpr (HALF) return h2f((uint16_t)(old[i] >> (16 * j)));
+          else return old[i][j];
+        });
+      }
+    }
   }
 }
 
@@ -633,13 +655,8 @@ extern "C" int hsg_gdn_tree_step(const void* qkv, int64_t qkv_stride, int32_t q_
   };
   const auto by_type = [&](auto nt) {
     constexpr int NT = decltype(nt)::value;
-    const auto by_state = [&](auto half) {
-      constexpr bool HALF = decltype(half)::value;
-      if (commits) z ? launch(gdn_tree_kernel<NT, HALF, true, true>) : launch(gdn_tree_kernel<NT, HALF, false, true>);
-      else z ? launch(gdn_tree_kernel<NT, HALF, true, false>) : launch(gdn_tree_kernel<NT, HALF, false, false>);
-    };
-    if (state_dtype == HSG_STATE_F16) by_state(std::true_type{});
-    else by_state(std::false_type{});
+    if (state_dtype == HSG_STATE_F16) z ? launch(gdn_tree_kernel<NT, true, true>) : launch(gdn_tree_kernel<NT, true, false>);
+    else z ? launch(gdn_tree_kernel<NT, false, true>) : launch(gdn_tree_kernel<NT, false, false>);
   };
   if (max_nodes <= 16) by_type(std::integral_constant<int, 1>{});
   else if (max_nodes <= 32) by_type(std::integral_constant<int, 2>{});
