@@ -204,8 +204,10 @@ __device__ __forceinline__ void walk_row(const TreeStepParams& p, const TreeRow&
   }
 }
 
-template <int NT, bool HALF, bool GATED>
-__global__ __launch_bounds__(64 * NW, NT == 1 ? 4 : NT == 2 ? 3 : 2) void gdn_tree_kernel(const TreeStepParams p) {
+// MOVES: rows may commit. Without, S0's registers are free as it is split, and trees of one tile over fp32 states have four
+// workgroups on a CU instead of three: 352 x 1 node 68 against 72 us.
+template <int NT, bool HALF, bool GATED, bool MOVES>
+__global__ __launch_bounds__(64 * NW, NT == 4 ? 2 : HALF || !MOVES ? 4 : 3) void gdn_tree_kernel(const TreeStepParams p) {
   constexpr int PARTS = HALF ? 2 : 3;
   __shared__ TreeStepLds<NT> lds;
   const int lane = threadIdx.x & 63;
@@ -213,7 +215,7 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 4 : NT == 2 ? 3 : 2) void gdn_tr
   const int g4 = lane >> 4, c = lane & 15;
   const int n = blockIdx.x / p.HV, hv = blockIdx.x - n * p.HV;
   const int64_t slot = p.slots[n], len64 = p.lens[n], off = p.offsets[n];
-  const int64_t done64 = p.commits ? p.commits[n] : 0;
+  const int64_t done64 = MOVES && p.commits ? p.commits[n] : 0;
   if ((slot < 0) | (slot >= p.state_rows) | (len64 <= 0) | (len64 > p.max_nodes)) return;
   const int len = (int)len64;
   const int tiles = (len + 15) >> 4;
@@ -533,7 +535,7 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 4 : NT == 2 ? 3 : 2) void gdn_tr
   }
 
   // ---- the committed chain moves the state: u scaled, split as the state was, times k^T read from LDS transposed ----
-  if (ro.done > 0) {
+  if (MOVES && ro.done > 0) {
     const float ec = lds.eG[ro.done - 1];
     constexpr int NP = (NT + 1) / 2;     // pairs of tiles: a product takes 32 nodes, the lane's own 4 of either tile
     bf16x8 up[NP][2][3];
@@ -589,28 +591,13 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? 4 : NT == 2 ? 3 : 2) void gdn_tr
         }
       }
     };
-    if constexpr (NT == 4) {   // LDS leaves two workgroups a CU, and them the registers to keep S0
+    // (through an empty asm: the values as converted and split for the products would be kept for this)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) move(s, [&](int j, int i) { return s0(s, j, i); });
-    } else {
-      // S0 again, from a cache, 32 rows at a time and the next ones on their way
-      const StatePair* const again = reinterpret_cast<const StatePair*>(state + lane_per_site(state_lane));
-      StatePair old[8], next[8];
+    for (int s = 0; s < 4; ++s) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) next[i] = again[i * (KD / 2)];
-#pragma unroll 1
-      for (int s = 0; s < 4; ++s) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) old[i] = next[i];
-        if (s < 3) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) next[i] = again[(32 * (s + 1) + i) * (KD / 2)];
-        }
-        move(s, [&](int j, int i) {
-          if constexpr (HALF) return h2f((uint16_t)(old[i] >> (16 * j)));
-          else return old[i][j];
-        });
-      }
+      for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(raw[s][i]));
+      move(s, [&](int j, int i) { return s0(s, j, i); });
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
@@ -655,8 +642,12 @@ extern "C" int hsg_gdn_tree_step(const void* qkv, int64_t qkv_stride, int32_t q_
   };
   const auto by_type = [&](auto nt) {
     constexpr int NT = decltype(nt)::value;
-    if (state_dtype == HSG_STATE_F16) z ? launch(gdn_tree_kernel<NT, true, true>) : launch(gdn_tree_kernel<NT, true, false>);
-    else z ? launch(gdn_tree_kernel<NT, false, true>) : launch(gdn_tree_kernel<NT, false, false>);
+    if (state_dtype == HSG_STATE_F16)
+      z ? launch(gdn_tree_kernel<NT, true, true, true>) : launch(gdn_tree_kernel<NT, true, false, true>);
+    else if (NT == 1 && !commits)
+      z ? launch(gdn_tree_kernel<1, false, true, false>) : launch(gdn_tree_kernel<1, false, false, false>);
+    else
+      z ? launch(gdn_tree_kernel<NT, false, true, true>) : launch(gdn_tree_kernel<NT, false, false, true>);
   };
   if (max_nodes <= 16) by_type(std::integral_constant<int, 1>{});
   else if (max_nodes <= 32) by_type(std::integral_constant<int, 2>{});
