@@ -57,11 +57,11 @@ struct TreeStepLds {
     struct {
       float A[N][PITCH];   // -A_ij
       float P[N][PITCH];
+      f32x4 T[NT][64];     // (I + A_bb)^-1 of the diagonal blocks, as the A operand of a lane
     };
     float U[N][KD];        // walk_row
   };
   uint16_t k[N * KD], q[N * KD];   // row by row, 16-byte pieces at kq_at
-  f32x4 T[NT][64];                 // (I + A_bb)^-1 of the diagonal blocks, as the A operand of a lane
   double G[N];
   uint64_t mask[N];                // ancestors and itself, within the row
   float g[N], beta[N], eG[N], kinv[N], qinv[N];
@@ -207,7 +207,7 @@ __device__ __forceinline__ void walk_row(const TreeStepParams& p, const TreeRow&
 // MOVES: rows may commit. Without, S0's registers are free as it is split, and trees of one tile over fp32 states have four
 // workgroups on a CU instead of three: 352 x 1 node 68 against 72 us.
 template <int NT, bool HALF, bool GATED, bool MOVES>
-__global__ __launch_bounds__(64 * NW, NT == 4 ? 2 : HALF || !MOVES ? 4 : 3) void gdn_tree_kernel(const TreeStepParams p) {
+__global__ __launch_bounds__(64 * NW, NT > 2 ? (HALF && NT == 3 ? 3 : 2) : HALF || !MOVES ? 4 : 3) void gdn_tree_kernel(const TreeStepParams p) {
   constexpr int PARTS = HALF ? 2 : 3;
   __shared__ TreeStepLds<NT> lds;
   const int lane = threadIdx.x & 63;
@@ -233,21 +233,19 @@ __global__ __launch_bounds__(64 * NW, NT == 4 ? 2 : HALF || !MOVES ? 4 : 3) void
 
   // Loads are waited for in the order of their issue: what the first phases need is loaded before S0, what the last ones need
   // after it.
-  // ---- k and q of a tile: with 4 tiles wave = tile; else waves from 0 on take k, waves from 2 on q ----
-  constexpr bool BOTH = NT == 4;
-  const int kt = BOTH ? wave : wave % NT;
-  const bool is_q = !BOTH && wave >= 2, idle = !BOTH && (wave & 1) >= NT;
-  // (lane offsets are 32 bits on a uniform base: 64-bit addresses per lane cost the registers that a third workgroup needs)
+  // ---- the tiles of k, then of q, dealt over the waves ----
+  constexpr int EACH = (2 * NT + NW - 1) / NW;
+  // (lane offsets are 32 bits on a uniform base: 64-bit addresses per lane cost the registers of a workgroup on the CU)
   const uint32_t stride = (uint32_t)p.qkv_stride;
-  const uint32_t kq_row = (uint32_t)min(16 * kt + c, len - 1) * stride + 8 * g4;
-  u32x4 kp[4], qp[BOTH ? 4 : 1];
-  if (!idle) {
-    const uint16_t* const src = is_q ? ro.q : ro.k;
+  u32x4 kq[EACH][4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      kp[s] = *reinterpret_cast<const u32x4*>(src + 32 * s + kq_row);
-      if constexpr (BOTH) qp[s] = *reinterpret_cast<const u32x4*>(ro.q + 32 * s + kq_row);
-    }
+  for (int e = 0; e < EACH; ++e) {
+    const int job = wave + NW * e;
+    if (job >= 2 * NT) break;
+    const uint16_t* const src = job >= NT ? ro.q : ro.k;
+    const uint32_t row = (uint32_t)min(16 * (job % NT) + c, len - 1) * stride + 8 * g4;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) kq[e][s] = *reinterpret_cast<const u32x4*>(src + 32 * s + row);
   }
   const int64_t node = off + min(lane, len - 1);
   uint64_t mask = 0;
@@ -296,25 +294,24 @@ __global__ __launch_bounds__(64 * NW, NT == 4 ? 2 : HALF || !MOVES ? 4 : 3) void
   __builtin_amdgcn_sched_barrier(0);   // the loads stay where they stand
 
   // ---- k and q to LDS, and their lengths ----
-  const auto stage = [&](const u32x4 (&x)[4], uint16_t* to) {
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int job = wave + NW * e;
+    if (job >= 2 * NT) break;
+    const bool is_q = job >= NT;
+    const int row = 16 * (job % NT) + c;
+    uint16_t* const to = is_q ? lds.q : lds.k;
     float ss = 0.f;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       float y[8];
-      unpack8(x[s], y);
+      unpack8(kq[e][s], y);
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(y[i], y[i], ss);
-      *reinterpret_cast<u32x4*>(to + kq_at(16 * kt + c, 4 * s + g4)) = x[s];
+      *reinterpret_cast<u32x4*>(to + kq_at(row, 4 * s + g4)) = kq[e][s];
     }
-    return add_xor32(add_xor16(ss));
-  };
-  if (!idle) {
-    const float ss = stage(kp, is_q ? lds.q : lds.k);
-    if (g4 == 0) (is_q ? lds.qinv : lds.kinv)[16 * kt + c] = (is_q ? p.scale : 1.0f) / sqrtf(ss + 1e-6f);
-    if constexpr (BOTH) {
-      const float qq = stage(qp, lds.q);
-      if (g4 == 0) lds.qinv[16 * kt + c] = p.scale / sqrtf(qq + 1e-6f);
-    }
+    ss = add_xor32(add_xor16(ss));
+    if (g4 == 0) (is_q ? lds.qinv : lds.kinv)[row] = (is_q ? p.scale : 1.0f) / sqrtf(ss + 1e-6f);
   }
   // ---- a node's scalars: lane = node ----
   if (wave == 0) {
@@ -575,7 +572,7 @@ __global__ __launch_bounds__(64 * NW, NT == 4 ? 2 : HALF || !MOVES ? 4 : 3) void
           };
           const u32x2 lo = four(2 * t2);
           u32x2 hi = {0u, 0u};
-          if (2 * t2 + 1 < NT) hi = four(min(2 * t2 + 1, NT - 1));
+          if (2 * t2 + 1 < NT) hi = four(2 * t2 + 1 < NT ? 2 * t2 + 1 : 0);
           const bf16x8 kf = __builtin_bit_cast(bf16x8, (u32x4){lo[0], lo[1], hi[0], hi[1]});
 #pragma unroll
           for (int w = 2; w >= 0; --w)
@@ -651,6 +648,7 @@ extern "C" int hsg_gdn_tree_step(const void* qkv, int64_t qkv_stride, int32_t q_
   };
   if (max_nodes <= 16) by_type(std::integral_constant<int, 1>{});
   else if (max_nodes <= 32) by_type(std::integral_constant<int, 2>{});
+  else if (max_nodes <= 48) by_type(std::integral_constant<int, 3>{});
   else by_type(std::integral_constant<int, 4>{});
   return launch_status();
 }
