@@ -62,7 +62,7 @@ struct TreeStepLds {
     float U[N][KD];        // walk_row
   };
   uint16_t k[N * KD], q[N * KD];   // row by row, 16-byte pieces at kq_at
-  double G[N];
+  double G[N];                     // the decay down to the node, as a power of 2
   uint64_t mask[N];                // ancestors and itself, within the row
   float g[N], beta[N], eG[N], kinv[N], qinv[N];
   float left[N];                   // e^(G_c - G_i) on the committed chain, else 0
@@ -317,10 +317,10 @@ __global__ __launch_bounds__(64 * NW, NT > 2 ? (HALF && NT == 3 ? 3 : 2) : HALF 
   if (wave == 0) {
     const bool valid = lane < len;
     const uint64_t self = 1ull << lane;
-    mask = valid ? (mask & (self - 1)) | self : self;
+    mask = valid ? (mask & (self - 1)) | self : 0ull;
     const float g = valid ? log_decay(a, a_log, dt) : 0.f;
     // the sum down the path, by pointer doubling
-    double sum = g;
+    double sum = (double)g * 1.4426950408889634;   // of 2
     const uint64_t above = mask & ~self;
     int up = above ? 63 - __clzll((long long)above) : -1;
     for (int far = 1; far < len; far <<= 1) {
@@ -335,8 +335,8 @@ __global__ __launch_bounds__(64 * NW, NT > 2 ? (HALF && NT == 3 ? 3 : 2) : HALF 
       lds.mask[lane] = mask;
       lds.g[lane] = g;
       lds.G[lane] = sum;
-      lds.eG[lane] = expf((float)sum);
-      lds.left[lane] = lane < ro.done ? expf((float)(Gc - sum)) : 0.f;
+      lds.eG[lane] = __builtin_amdgcn_exp2f((float)sum);
+      lds.left[lane] = lane < ro.done ? __builtin_amdgcn_exp2f((float)(Gc - sum)) : 0.f;
       lds.beta[lane] = valid ? sigmoid_f32(b) : 0.f;
     }
   }
@@ -344,18 +344,26 @@ __global__ __launch_bounds__(64 * NW, NT > 2 ? (HALF && NT == 3 ? 3 : 2) : HALF 
 
   const auto k_part = [&](int t, int s) { return load_bf16x8(&lds.k[kq_at(16 * t + c, 4 * s + g4)]); };
   const auto q_part = [&](int t, int s) { return load_bf16x8(&lds.q[kq_at(16 * t + c, 4 * s + g4)]); };
-  // ---- -A and P, block pairs dealt over the waves ----
-  for (int pair = wave; pair < NT * (NT + 1) / 2; pair += NW) {
-    const int bi = pair < 1 ? 0 : pair < 3 ? 1 : pair < 6 ? 2 : 3;
-    const int bj = pair - bi * (bi + 1) / 2;
+  // ---- -A and P, block pairs dealt over the waves: every pair's products are issued before the first is used ----
+  constexpr int PAIRS = (NT * (NT + 1) / 2 + NW - 1) / NW;
+  const auto row_block = [](int pair) { return pair < 1 ? 0 : pair < 3 ? 1 : pair < 6 ? 2 : pair < 10 ? 3 : NT; };
+  f32x4 kk[PAIRS], qk[PAIRS];
+#pragma unroll
+  for (int e = 0; e < PAIRS; ++e) {
+    const int pair = wave + NW * e, bi = row_block(pair), bj = pair - bi * (bi + 1) / 2;
     if (bi >= tiles) break;
-    f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = {0.f, 0.f, 0.f, 0.f};
+    kk[e] = qk[e] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const bf16x8 y = k_part(bj, s);
-      kk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k_part(bi, s), y, kk, 0, 0, 0);
-      qk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q_part(bi, s), y, qk, 0, 0, 0);
+      kk[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k_part(bi, s), y, kk[e], 0, 0, 0);
+      qk[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q_part(bi, s), y, qk[e], 0, 0, 0);
     }
+  }
+#pragma unroll
+  for (int e = 0; e < PAIRS; ++e) {
+    const int pair = wave + NW * e, bi = row_block(pair), bj = pair - bi * (bi + 1) / 2;
+    if (bi >= tiles) break;
     const int j = 16 * bj + c, i0 = 16 * bi + 4 * g4;
     const double Gj = lds.G[j];
     const float kj = lds.kinv[j];
@@ -364,10 +372,10 @@ __global__ __launch_bounds__(64 * NW, NT > 2 ? (HALF && NT == 3 ? 3 : 2) : HALF 
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = i0 + r;
-      const bool on = (lds.mask[i] >> j & 1) && i < len;
-      const float d = expf((float)(lds.G[i] - Gj)) * kj;
-      lds.P[i][j] = on ? qi[r] * d * qk[r] : 0.f;
-      lds.A[i][j] = on && i != j ? -be[r] * ki[r] * d * kk[r] : 0.f;
+      const bool on = lds.mask[i] >> j & 1;
+      const float d = __builtin_amdgcn_exp2f((float)(lds.G[i] - Gj)) * kj;
+      lds.P[i][j] = on ? qi[r] * d * qk[e][r] : 0.f;
+      lds.A[i][j] = on && i != j ? -be[r] * ki[r] * d * kk[e][r] : 0.f;
     }
   }
   lds_barrier();
