@@ -393,8 +393,10 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
       for (int i = 0; i < 4; ++i) {
         const float p0 = exp2_fast(__builtin_fmaf(S[t][i >> 1][2 * (i & 1)], sl2, -base));
         const float p1 = exp2_fast(__builtin_fmaf(S[t][i >> 1][2 * (i & 1) + 1], sl2, -base));
-        sum[t] += p0 + p1;
         w[i] = pack_bf16x2(p0, p1);
+        float q0, q1;
+        unpack2(w[i], q0, q1);   // the weights as rounded: what dominates a row keeps no rounding
+        sum[t] += q0 + q1;
       }
       pb[t] = as_bf16x8(w);
     }
