@@ -43,6 +43,7 @@ constexpr int BLOCKS = W_MAX / KB + MOST / KB;
 constexpr int KP_NONE = -(1 << 30);    // an empty ring column
 constexpr int KP_FAR = 1 << 29;        // clamp of a position relative to the row's start
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int SPLITS_MAX = 8;          // workgroups that split a row's key blocks
 constexpr float SLACK = 8.f;           // log2 of how far a score may exceed the running maximum before it is moved
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
@@ -644,7 +645,6 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
 }
 
 // Joins the splits' partial sums: a wave a query row, 4 dims a lane; every split's loads are in flight at once
-constexpr int SPLITS_MAX = 8;
 __global__ __launch_bounds__(256) void tree_attn_join_kernel(const TreeAttnParams p) {
   const int pair = blockIdx.x;
   const int n = pair / p.hkv, h = pair - n * p.hkv;
@@ -724,18 +724,26 @@ __global__ __launch_bounds__(256) void tree_ring_write_kernel(const TreeAttnPara
   }
 }
 
-// Query rows of a workgroup: from 65 on every wave has its own and the keys pass through LDS
-inline int rows_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 64 ? 64 : 128; }
+// Query rows of a workgroup. Up to 16 the waves split their keys (352 x 1 node 124 us, against 140 through LDS); beyond, keys
+// pass through LDS for 4 waves of one tile, or of two where that fills the chip (256 CUs) and wastes little: a workgroup of
+// 128 rows takes 1.5 times as long as one of 64. 64 x 64 nodes, 16 q / 4 kv heads: 68 us with 128 rows, 88 with 64; 20 x 64
+// 44 and 38; 100 x 33 (129 to 192 rows are three workgroups of 64) 109 and 86.
+inline int rows_of(int64_t pairs, int64_t rows) {
+  if (rows <= 64) return rows <= 16 ? 16 : 64;
+  return (rows + 63) / 64 == 3 || pairs * ((rows + 127) / 128) < 256 ? 64 : 128;
+}
 
-// Workgroups of a row's key blocks: few rows leave the chip (256 CUs) short of workgroups, and one CU moves only a few tens
-// of GB/s. 8 at most.
-inline int splits_of(int64_t n_rows, int64_t hkv, int64_t rows) {
-  const int64_t units = n_rows * hkv * ((rows + rows_of(rows) - 1) / rows_of(rows));
+// Workgroups of a row's key blocks: few rows leave the chip short of workgroups, and one CU moves only a few tens of GB/s.
+// Twice as many for twice as many units were no faster: 30 x 14 nodes (120 units) 21 us with 2 and with 4, 60 x 14 42 us with 1
+// against 33 and a join of 12 with 2.
+inline int splits_of(int64_t pairs, int64_t rows) {
+  const int per = rows_of(pairs, rows);
+  const int64_t units = pairs * ((rows + per - 1) / per);
   return units <= 32 ? SPLITS_MAX : units <= 64 ? 4 : units <= 128 ? 2 : 1;
 }
 
-inline size_t part_bytes(int64_t n_rows, int64_t hkv, int64_t rows, int splits) {
-  return splits == 1 ? 0 : (size_t)(n_rows * hkv * splits * rows) * (D + 2) * sizeof(float);
+inline size_t part_bytes(int64_t pairs, int64_t rows, int splits) {
+  return splits == 1 ? 0 : (size_t)(pairs * splits * rows) * (D + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -745,7 +753,8 @@ extern "C" size_t hsg_tree_attention_workspace_bytes(int32_t n_rows, int32_t hkv
   using namespace hsg;
   if (n_rows <= 0 || hkv <= 0 || groups <= 0 || max_nodes <= 0 || max_nodes > MOST) return 0;
   const int64_t rows = (int64_t)groups * max_nodes;
-  return part_bytes(n_rows, hkv, rows, splits_of(n_rows, hkv, rows));
+  const int64_t pairs = (int64_t)n_rows * hkv;
+  return part_bytes(pairs, rows, splits_of(pairs, rows));
 }
 
 extern "C" int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int64_t q_sg, void* ring_k, void* ring_v,
@@ -775,7 +784,7 @@ extern "C" int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int
     return HSG_ERR_ALIGN;
   const int64_t rows = (int64_t)groups * max_nodes;
   const int64_t pairs = (int64_t)n_rows * hkv;
-  const int per_wg = rows_of(rows);
+  const int per_wg = rows_of(pairs, rows);
   TreeAttnParams p{};
   p.q = static_cast<const uint16_t*>(q); p.q_sl = q_sl; p.q_sh = q_sh; p.q_sg = q_sg;
   p.ring_k = static_cast<uint16_t*>(ring_k); p.ring_v = static_cast<uint16_t*>(ring_v);
@@ -789,8 +798,8 @@ extern "C" int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int
   if (pairs >= (1 << 24) || rows >= (1 << 20)) return HSG_ERR_SHAPE;
   p.pairs = (int)pairs;
   p.qblocks = (int)((rows + per_wg - 1) / per_wg);
-  p.splits = splits_of(n_rows, hkv, rows);
-  if (!workspace || workspace_bytes < part_bytes(n_rows, hkv, rows, p.splits)) p.splits = 1;
+  p.splits = splits_of(pairs, rows);
+  if (!workspace || workspace_bytes < part_bytes(pairs, rows, p.splits)) p.splits = 1;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.splits > 1 ? p.part_o + pairs * p.splits * rows * D : nullptr;
   p.out = static_cast<uint16_t*>(out); p.o_sl = o_sl; p.o_sh = o_sh; p.o_sg = o_sg;

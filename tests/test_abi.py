@@ -221,6 +221,6 @@ def test_tree_operators_refuse_before_launch():
                     ({"ws": 264, "ws_bytes": 1 << 30}, ALIGN)):
         assert attend(**bad) == rc, bad
     need = L.hsg_tree_attention_workspace_bytes
-    assert need(1, 4, 4, 12) == 4 * 4 * 48 * 258 * 4      # 4 kv heads, 4 splits, 48 query rows of 256 sums, maximum, weight
+    assert need(1, 4, 4, 12) == 4 * 8 * 48 * 258 * 4      # 4 kv heads, 8 splits, 48 query rows of 256 sums, maximum, weight
     assert need(20, 4, 4, 12) == 20 * 4 * 2 * 48 * 258 * 4
     assert need(352, 4, 4, 12) == 0 and need(0, 4, 4, 12) == 0 and need(1, 4, 4, 65) == 0
