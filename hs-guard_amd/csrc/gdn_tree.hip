@@ -619,7 +619,7 @@ extern "C" int hsg_gdn_tree_step(const void* qkv, int64_t qkv_stride, int32_t q_
                                  void* out, void* stream) {
   using namespace hsg;
   if (n_rows < 0 || state_rows <= 0 || H <= 0 || HV <= 0 || HV % H) return HSG_ERR_ARG;
-  if (state_dtype != HSG_STATE_F32 && state_dtype != HSG_STATE_F16) return HSG_ERR_ARG;
+  if ((state_dtype != HSG_STATE_F32 && state_dtype != HSG_STATE_F16) || !isfinite(scale)) return HSG_ERR_ARG;
   if (K != KD || V != KD || max_nodes <= 0 || max_nodes > HSG_TREE_MAX_NODES) return HSG_ERR_SHAPE;
   if (n_rows == 0) return HSG_OK;
   if (!qkv || !a || !b || !A_log || !dt_bias || !state || !slots || !lens || !offsets || !masks || !out ||

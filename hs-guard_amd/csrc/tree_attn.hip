@@ -24,8 +24,9 @@
 // Where few rows leave the chip short of workgroups, workgroups split a row's key blocks further and a second launch joins
 // their partial sums: a lone row of 12 nodes 12.7 + 8.6 us.
 //
-// A masked pair has P = 0, which would carry a NaN or an infinity of a value to queries that do not see it: a query row with a
-// result that is not finite is computed again from the keys that it sees alone (walk_keys).
+// A masked pair has P = 0, which would carry a NaN or an infinity of a value to queries that do not see it: columns that no
+// query of the row sees are not read (another key's are, in their place), and a query row with a result that is not finite is
+// computed again from the keys that it sees alone (walk_keys).
 #include <math.h>
 #include <stddef.h>
 
@@ -243,7 +244,8 @@ struct TreeAttnLds {
   };
   int kp[W_MAX + MOST];       // places of the ring's keys before the start; then the nodes' depths
   uint64_t mask[MOST];        // the nodes' ancestors and themselves
-  uint32_t flags[BLOCKS];     // bit 0: some query may see a key of the block; 1: all see all
+  uint32_t live[BLOCKS];      // per block: the keys that some query of the row sees; a block's other columns hold anything
+  uint32_t whole[BLOCKS];     // every query sees every key
   float ml[NW][T][16][2];
   uint32_t odd[QW * T];       // query rows with a result that is not finite
   __device__ TreeAttnLds() {}
@@ -303,10 +305,12 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
   for (int col = threadIdx.x; col < W_MAX; col += 64 * NW) {
     const int place = col < W ? key_place(ro.ring_pos[min(col, W - 1)], ro.start) : KP_NONE;
     lds.kp[col] = place;
-    const uint64_t some = __ballot(place > -W), all = __ballot(place > len - 1 - W);
+    const uint64_t live = __ballot(place > -W), whole = __ballot(place > len - 1 - W);
     if (lane == 0) {
-      lds.flags[col / KB] = ((uint32_t)some ? 1u : 0u) | ((uint32_t)all == ~0u ? 2u : 0u);
-      lds.flags[col / KB + 1] = ((uint32_t)(some >> 32) ? 1u : 0u) | ((uint32_t)(all >> 32) == ~0u ? 2u : 0u);
+      lds.live[col / KB] = (uint32_t)live;
+      lds.live[col / KB + 1] = (uint32_t)(live >> 32);
+      lds.whole[col / KB] = (uint32_t)whole == ~0u;
+      lds.whole[col / KB + 1] = (uint32_t)(whole >> 32) == ~0u;
     }
   }
   if (threadIdx.x < MOST) {
@@ -315,6 +319,10 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
     lds.kp[W_MAX + threadIdx.x] = (int)__popcll(mask) - 1;
   }
   if (threadIdx.x < QW * T) lds.odd[threadIdx.x] = 0u;
+  const auto live_nodes = [&](int b) {   // of the tree's block b
+    const int n = len - (b - RB) * KB;
+    return n >= KB ? ~0u : (1u << n) - 1u;
+  };
   __syncthreads();
 
   // ---- the wave's key blocks ----
@@ -333,9 +341,8 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
   // bit b: the wave takes block b, which some query may see; and of these the ones that all see whole
   uint32_t rest = 0u, whole;
   {
-    const uint32_t f = lane < RB ? lds.flags[lane] : 0u;
-    const uint32_t some = (uint32_t)__ballot((f & 1u) != 0u) | (~0u << RB);
-    whole = (uint32_t)__ballot((f & 2u) != 0u);
+    const uint32_t some = (uint32_t)__ballot(lane < RB && lds.live[min(lane, BLOCKS - 1)] != 0u) | (~0u << RB);
+    whole = (uint32_t)__ballot(lane < RB && lds.whole[min(lane, BLOCKS - 1)] != 0u);
     for (int b = b_first; b < n_blocks; b += step) rest |= some & (1u << b);
     if (tiles == 0 && KW > 1) rest = 0u;
   }
@@ -420,14 +427,16 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
     // keys and values straight from memory to the operand registers: a block's values are loaded before its scores, the next
     // block's keys after them
     u32x4 kr[2][D / 32], vr[2][8];
+    // a key that no query sees is read as one that is
+    const auto live_of = [&](int b) { return b < RB ? __builtin_amdgcn_readfirstlane(lds.live[b]) : live_nodes(b); };
+    const auto seen_row = [](uint32_t live, int r) { return (uint32_t)(live >> r & 1u ? r : __builtin_ctz(live)); };
     const auto load_keys = [&](int b) __attribute__((always_inline)) {
       const bool ring = b < RB;
       const uint16_t* base = ring ? ro.ring_k + b * (KB * D) : ro.k + (int64_t)(b - RB) * KB * p.nk_sl;
-      const uint32_t st = ring ? D : (uint32_t)p.nk_sl;
-      const int last = ring ? KB - 1 : len - 1 - (b - RB) * KB;
+      const uint32_t st = ring ? D : (uint32_t)p.nk_sl, live = live_of(b);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const uint32_t off = 2 * ((uint32_t)min(16 * kt + c, last) * st + 8 * g4);
+        const uint32_t off = 2 * (seen_row(live, 16 * kt + c) * st + 8 * g4);
 #pragma unroll
         for (int ks = 0; ks < D / 32; ++ks) kr[kt][ks] = load16_at(base + 32 * ks, off);
       }
@@ -438,11 +447,10 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
       const bool ring = b < RB;
       {
         const uint16_t* base = ring ? ro.ring_v + b * (KB * D) : ro.v + (int64_t)(b - RB) * KB * p.nv_sl;
-        const uint32_t st = ring ? D : (uint32_t)p.nv_sl;
-        const int last = ring ? KB - 1 : len - 1 - (b - RB) * KB;
+        const uint32_t st = ring ? D : (uint32_t)p.nv_sl, live = live_of(b);
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
-          const uint32_t off = 2 * ((uint32_t)min(16 * (s >> 2) + 4 * g4 + (s & 3), last) * st + 8 * c);
+          const uint32_t off = 2 * (seen_row(live, 16 * (s >> 2) + 4 * g4 + (s & 3)) * st + 8 * c);
           vr[0][s] = load16_at(base, off);
           vr[1][s] = load16_at(base + 128, off);
         }
@@ -480,19 +488,21 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
       const int row = wave * EACH + (l >> 5);
       const uint32_t k_piece = 16 * ((l & 31) ^ (row & 15)), v_piece = 16 * (l & 31);
       // (the rows of a wave share all but bits 1 and 2, which 2 e sets)
-      if (ring) {
+      if (whole >> b & 1u) {
         const uint32_t k_off = row * (2 * D) + k_piece, v_off = row * (2 * D) + v_piece;
 #pragma unroll
         for (int e = 0; e < EACH / 2; ++e) {
           load_lds16(kb + 2 * e * D, k_off ^ (32 * e), to + 1024 * e);
           load_lds16(vb + 2 * e * D, v_off, to + (uint32_t)offsetof(KeyStage, v) + 1024 * e);
         }
-      } else {
+      } else {   // a key that no query sees is read as one that is
+        const uint32_t live = ring ? __builtin_amdgcn_readfirstlane(lds.live[b]) : live_nodes(b);
+        const uint32_t k_st = ring ? 2 * D : (uint32_t)(2 * p.nk_sl), v_st = ring ? 2 * D : (uint32_t)(2 * p.nv_sl);
 #pragma unroll
         for (int e = 0; e < EACH / 2; ++e) {
-          const uint32_t at = (uint32_t)min(row + 2 * e, len - 1 - (b - RB) * KB);
-          load_lds16(kb, at * (uint32_t)(2 * p.nk_sl) + (k_piece ^ (32 * e)), to + 1024 * e);
-          load_lds16(vb, at * (uint32_t)(2 * p.nv_sl) + v_piece, to + (uint32_t)offsetof(KeyStage, v) + 1024 * e);
+          const uint32_t at = live >> (row + 2 * e) & 1u ? (uint32_t)(row + 2 * e) : (uint32_t)__builtin_ctz(live);
+          load_lds16(kb, at * k_st + (k_piece ^ (32 * e)), to + 1024 * e);
+          load_lds16(vb, at * v_st + v_piece, to + (uint32_t)offsetof(KeyStage, v) + 1024 * e);
         }
       }
     };
@@ -616,8 +626,8 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
         const float inv = 1.0f / total;
 #pragma unroll
         for (int e = 0; e < 8 * R; ++e) y[e] *= inv;
-        if (!all_finite(y)) atomicOr(&lds.odd[wq * T + t], 1u << ce);
-        store_gated(p, ro, row, d0, y, gw[STAGED ? 0 : t][x]);
+        if (all_finite(y)) store_gated(p, ro, row, d0, y, gw[STAGED ? 0 : t][x]);
+        else atomicOr(&lds.odd[wq * T + t], 1u << ce);
       } else {
         const int64_t at = ((int64_t)pair * p.splits + split) * ((int64_t)G * p.max_nodes) + row;
         float* dst = p.part_o + at * D + d0;
@@ -632,7 +642,7 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
   }
   if (p.splits > 1) return;
   // ---- query rows with a result that is not finite: again, over the keys that they see alone ----
-  __syncthreads();   // also: the stores of these rows' first results are done
+  __syncthreads();
   for (int i = threadIdx.x >> 5; i < ROWS; i += 64 * NW / 32)
     if (lds.odd[i >> 4] >> (i & 15) & 1u) {
       const int d0 = 8 * (threadIdx.x & 31);
@@ -770,6 +780,7 @@ extern "C" int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int
   if (n_rows < 0 || hkv <= 0 || groups <= 0 || ring_rows <= 0) return HSG_ERR_ARG;
   if (head_dim != D || window <= 0 || window > W_MAX || window % KB != 0 || max_nodes <= 0 || max_nodes > MOST)
     return HSG_ERR_SHAPE;
+  if (!isfinite(scale)) return HSG_ERR_ARG;
   if (n_rows == 0) return HSG_OK;
   if (!q || !ring_k || !ring_v || !new_k || !new_v || !ring_pos || !slots || !starts || !lens || !offsets || !masks || !out)
     return HSG_ERR_ARG;

@@ -440,6 +440,8 @@ def tree_conv_silu(qkv, pool, weight, slots, trees):
         raise AssertionError("tree_conv_silu: pool [S, K-1, C], weight [C, 1, K]")
     n = _tree_rows(trees, slots, total)
     out = qkv.new_empty((total, c))
+    if not total:
+        return out
     _launch("hsg_tree_conv_silu", device, qkv.data_ptr(), stride, pool.data_ptr(), pool.shape[0], weight.data_ptr(), ks,
             slots.data_ptr(), trees.lens.data_ptr(), trees.offsets.data_ptr(), _ptr(trees.commits), trees.masks.data_ptr(),
             n, trees.max_nodes, c, out.data_ptr(), c)
@@ -474,6 +476,8 @@ def gdn_tree_step(packed, key_dim, heads, head_k, value_heads, head_v, a, b, A_l
         _require(norm_weight.numel() == head_v, "norm_weight must be [V]")
     n = _tree_rows(trees, slots, total)
     out = packed.new_empty((total, hvv))
+    if not total:
+        return out
     _launch("hsg_gdn_tree_step", device, packed.data_ptr(), stride, 0, key_dim, 2 * key_dim, a.data_ptr(), b.data_ptr(), ab,
             A_log.data_ptr(), dt_bias.data_ptr(), state.data_ptr(), _STATE_CODES[state.dtype], state.shape[0],
             slots.data_ptr(), trees.lens.data_ptr(), trees.offsets.data_ptr(), _ptr(trees.commits), trees.masks.data_ptr(),
@@ -508,6 +512,8 @@ def tree_ring_attention(q, ring_k, ring_v, new_k, value, gate, ring_pos, slots, 
     n = _tree_rows(trees, slots, total)
     _require(starts.shape == slots.shape, "starts must be [n]")
     out = q.new_empty((total, hq * d))
+    if not total:
+        return out
     most = trees.max_nodes
     if workspace is None:
         need = lib().hsg_tree_attention_workspace_bytes(n, hkv, groups, most)

@@ -560,7 +560,9 @@ int hsg_tree_conv_silu(const void* x, int64_t x_stride, void* pool, int64_t pool
  *   z == NULL: out = bf16(o), and norm_w and eps are not read.
  *   qkv, a, b, A_log, dt_bias, state, z, norm_w, out as hsg_gdn_slot_step_gated's. Rows with commits[n] > 0 move the state
  *   by their chain; no other state is written. A NaN or an infinity reaches its node and that node's descendants alone.
- * Supported: K == V == 128, HV % H == 0; qkv and its offsets and stride 16-byte aligned.
+ *   out must not overlap an input.
+ * Supported: K == V == 128, HV % H == 0 and HV < 65536; qkv and its offsets and stride 16-byte aligned, the strides of qkv
+ * and z below 2^24; a finite scale.
  */
 int hsg_gdn_tree_step(const void* qkv, int64_t qkv_stride, int32_t q_off, int32_t k_off, int32_t v_off, const void* a,
                       const void* b, int64_t ab_stride, const void* A_log, const void* dt_bias, void* state,
@@ -576,10 +578,13 @@ int hsg_gdn_tree_step(const void* qkv, int64_t qkv_stride, int32_t q_off, int32_
  * bf16 for their product. gate may be NULL: no gating. Element addresses, ring pools and ring_pos as hsg_ring_attention's
  * packed layout. Rows with commits[n] > 0 write their chain's keys and values into the ring columns (starts[n] + j) % window
  * (of a chain longer than the window the last `window`), in a launch after the reads; ring_pos is the caller's
- * (hsg_ring_pos_update with lens = commits). A NaN or an infinity reaches only the nodes that see it.
+ * (hsg_ring_pos_update with lens = commits). A NaN or an infinity reaches only the nodes that see it. out must not overlap
+ * an input.
  * workspace (optional): with at least hsg_tree_attention_workspace_bytes(n_rows, hkv, groups, max_nodes) bytes (0: none is
- * used), 16-byte aligned, calls of few rows split a row's keys over workgroups; its contents need no initialisation.
- * Supported: head_dim == 256, window <= 512 and a multiple of 32; strides multiples of 8, pointers 16-byte aligned.
+ * used), 16-byte aligned, calls of few rows split a row's keys over workgroups; its contents need no initialisation, and
+ * calls that may run at once need one each.
+ * Supported: head_dim == 256, window <= 512 and a multiple of 32; strides multiples of 8, those of new_k's and new_v's
+ * tokens from 0 to 2^24 - 1, pointers 16-byte aligned; a finite scale.
  */
 size_t hsg_tree_attention_workspace_bytes(int32_t n_rows, int32_t hkv, int32_t groups, int32_t max_nodes);
 int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int64_t q_sg, void* ring_k, void* ring_v,

@@ -77,7 +77,7 @@ def signed(masks):
     return [m - (1 << 64) if m >> 63 else m for m in masks]
 
 
-LENS = [[1], [64], [1, 1, 1], [12, 0, 33, 1, 16, 17, 64], [8] * 9, [15, 16, 17, 31, 32, 33]]
+LENS = [[1], [64], [0, 0], [1, 1, 1], [12, 0, 33, 1, 16, 17, 64], [8] * 9, [15, 16, 17, 31, 32, 33]]
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -375,6 +375,8 @@ def test_attention_keeps_a_bad_value_to_who_sees_it(n, G, value):
     s["ring_v"][1, :, 300:] = value
     out = attention_call(s, dev, maps_of(dev, n), W, 0.0625)
     within(out, want, slack, 2.0 ** -8, "dead ring columns")
+    clean = {**s, "ring_k": s["ring_k"].nan_to_num(0, 0), "ring_v": s["ring_v"].nan_to_num(0, 0)}
+    assert torch.equal(out, attention_call(clean, dev, maps_of(dev, n), W, 0.0625)), "dead ring columns are not read"
     below = [i for i in range(n) if bad in tree.path(parents, i)]
     rest = [i for i in range(n) if i not in below]
     for name, seen in (("value", below), ("new_k", below), ("q", [bad])):
@@ -551,6 +553,9 @@ def test_refusals():
                 {"packed": s["packed"][:, :-8]}):
         with pytest.raises((AssertionError, ValueError)):
             gdn_call({**s, **bad}, 2, 2, dev["slots"], trees, bad.get("state", s["state"]))
+    for bad in (float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            attention_call(s, dev, trees, 512, bad)
     for bad in ({"q": s["q"][:, :, :128]}, {"ring_k": s["ring_k"][:, :, :-1]}, {"ring_pos": s["ring_pos"][:, :-1]},
                 {"new_k": s["new_k"].transpose(0, 1)}, {"gate": s["gate"][:, :-8]}):
         with pytest.raises((AssertionError, ValueError)):
