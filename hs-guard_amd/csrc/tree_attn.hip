@@ -109,6 +109,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// sigmoid to a few fp32 steps (its product is rounded to bf16), 4 instructions against the exact one's 16: an epilogue of 2
+// tiles holds 64 a lane
+__device__ __forceinline__ float gate_of(float x) { return __builtin_amdgcn_rcpf(1.0f + exp2_fast(-LOG2E * x)); }
 
 // node i's ancestors and itself
 __device__ __forceinline__ uint64_t mask_of(const int64_t* masks, int i) {
@@ -201,7 +204,7 @@ __device__ __forceinline__ void store_gated(const TreeAttnParams& p, const TreeK
       float gt[8];
       unpack8(gw[e], gt);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[8 * e + i] *= sigmoidf_(gt[i]);
+      for (int i = 0; i < 8; ++i) y[8 * e + i] *= gate_of(gt[i]);
     }
   }
 #pragma unroll
@@ -224,8 +227,16 @@ __device__ __forceinline__ void load_lds16(const void* base, uint32_t off, uint3
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
 }
 
-// Rows of 512 bytes, each loaded whole. The 16-byte pieces of a key are permuted by its number (piece pc of row r at pc ^ r %
-// 16), so that the scores' operand, one piece of 16 rows, spreads over the banks; of a value 16 pieces of a row are read.
+// LDS transpose read: within each group of 16 lanes, lane 4 q + e receives element e of the 4-value vectors that lanes q, q + 4,
+// q + 8 and q + 12 of its group address
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+__device__ __forceinline__ u32x2 ld_tr4(const uint16_t* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p)));
+}
+
+// Rows of 512 bytes, each loaded whole. The 16-byte pieces of a row are permuted by its number (piece pc of row r at pc ^ r %
+// 16), so that the scores' operand, one piece of 16 rows, and the values' transpose reads, 4 pieces of 16 rows, spread over
+// the banks.
 struct KeyStage {
   uint16_t k[KB][D];
   uint16_t v[KB][D];
@@ -284,6 +295,10 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
   const int b_first = wk + KW * split;                      // the first of the wave's blocks
 
   // ---- queries, and places of the keys ----
+  int64_t ring_pos[W_MAX / (64 * NW)];
+#pragma unroll
+  for (int e = 0; e < W_MAX / (64 * NW); ++e) ring_pos[e] = ro.ring_pos[min((int)threadIdx.x + 64 * NW * e, W - 1)];
+  const uint64_t mask = threadIdx.x < MOST ? mask_of(ro.masks, min((int)threadIdx.x, len - 1)) : 0ull;
   bf16x8 qr[STAGED ? T : 1][D / 32];
   int node[T];
 #pragma unroll
@@ -302,8 +317,51 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
         lds.q[wq * T + t][wk * (D / 32 / KW) + ks][lane] = load16(src + 32 * (wk * (D / 32 / KW) + ks));
     }
   }
-  for (int col = threadIdx.x; col < W_MAX; col += 64 * NW) {
-    const int place = col < W ? key_place(ro.ring_pos[min(col, W - 1)], ro.start) : KP_NONE;
+  const auto live_nodes = [&](int b) {   // of the tree's block b
+    const int n = len - (b - RB) * KB;
+    return n >= KB ? ~0u : (1u << n) - 1u;
+  };
+  // a key that no query sees is read as one that is
+  const auto live_of = [&](int b) { return b < RB ? __builtin_amdgcn_readfirstlane(lds.live[b]) : live_nodes(b); };
+  const auto seen_row = [](uint32_t live, int r) { return (uint32_t)(live >> r & 1u ? r : __builtin_ctz(live)); };
+  // (STAGED) block b's keys and values on their way into a stage
+  constexpr int EACH = 2 * KB * D * 2 / 1024 / NW;      // a wave's loads of a block
+  const auto fetch = [&](int b, int stage, bool all) __attribute__((always_inline)) {
+    const bool ring = b < RB;
+    const uint16_t* kb = ring ? ro.ring_k + b * (KB * D) : ro.k + (int64_t)(b - RB) * KB * p.nk_sl;
+    const uint16_t* vb = ring ? ro.ring_v + b * (KB * D) : ro.v + (int64_t)(b - RB) * KB * p.nv_sl;
+    const uint32_t to = lds_offset(&lds.stage[stage]) + 1024 * (EACH / 2) * wave;
+    // load e of the wave brings rows 2 o and 2 o + 1 of keys and values, o = wave * (EACH / 2) + e
+    const int l = lane_per_site(lane);
+    const int row = wave * EACH + (l >> 5);
+    const uint32_t piece = 16 * ((l & 31) ^ (row & 15));   // (the rows of a wave share all but bits 1 and 2, which 2 e sets)
+    if (all) {
+      const uint32_t off = row * (2 * D) + piece;
+#pragma unroll
+      for (int e = 0; e < EACH / 2; ++e) {
+        load_lds16(kb + 2 * e * D, off ^ (32 * e), to + 1024 * e);
+        load_lds16(vb + 2 * e * D, off ^ (32 * e), to + (uint32_t)offsetof(KeyStage, v) + 1024 * e);
+      }
+    } else {
+      const uint32_t live = live_of(b);
+      const uint32_t k_st = ring ? 2 * D : (uint32_t)(2 * p.nk_sl), v_st = ring ? 2 * D : (uint32_t)(2 * p.nv_sl);
+#pragma unroll
+      for (int e = 0; e < EACH / 2; ++e) {
+        const uint32_t at = seen_row(live, row + 2 * e);
+        load_lds16(kb, at * k_st + (piece ^ (32 * e)), to + 1024 * e);
+        load_lds16(vb, at * v_st + (piece ^ (32 * e)), to + (uint32_t)offsetof(KeyStage, v) + 1024 * e);
+      }
+    }
+  };
+  // the tree's first block, which needs nothing of the maps, is on its way first
+  const bool tree_first = STAGED && (RB - b_first) % step == 0;
+  if constexpr (STAGED) {
+    if (tree_first) fetch(RB, 0, false);
+  }
+#pragma unroll
+  for (int e = 0; e < W_MAX / (64 * NW); ++e) {
+    const int col = threadIdx.x + 64 * NW * e;
+    const int place = col < W ? key_place(ring_pos[e], ro.start) : KP_NONE;
     lds.kp[col] = place;
     const uint64_t live = __ballot(place > -W), whole = __ballot(place > len - 1 - W);
     if (lane == 0) {
@@ -314,16 +372,12 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
     }
   }
   if (threadIdx.x < MOST) {
-    const uint64_t mask = mask_of(ro.masks, min((int)threadIdx.x, len - 1));
     lds.mask[threadIdx.x] = mask;
     lds.kp[W_MAX + threadIdx.x] = (int)__popcll(mask) - 1;
   }
   if (threadIdx.x < QW * T) lds.odd[threadIdx.x] = 0u;
-  const auto live_nodes = [&](int b) {   // of the tree's block b
-    const int n = len - (b - RB) * KB;
-    return n >= KB ? ~0u : (1u << n) - 1u;
-  };
-  __syncthreads();
+  if constexpr (STAGED) lds_barrier();   // (the block's loads stay in flight)
+  else __syncthreads();
 
   // ---- the wave's key blocks ----
   const float sl2 = fmaxf(fabsf(p.scale) * LOG2E, 1e-37f);   // (not 0: a masked score is -inf)
@@ -427,9 +481,6 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
     // keys and values straight from memory to the operand registers: a block's values are loaded before its scores, the next
     // block's keys after them
     u32x4 kr[2][D / 32], vr[2][8];
-    // a key that no query sees is read as one that is
-    const auto live_of = [&](int b) { return b < RB ? __builtin_amdgcn_readfirstlane(lds.live[b]) : live_nodes(b); };
-    const auto seen_row = [](uint32_t live, int r) { return (uint32_t)(live >> r & 1u ? r : __builtin_ctz(live)); };
     const auto load_keys = [&](int b) __attribute__((always_inline)) {
       const bool ring = b < RB;
       const uint16_t* base = ring ? ro.ring_k + b * (KB * D) : ro.k + (int64_t)(b - RB) * KB * p.nk_sl;
@@ -477,44 +528,16 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
     }
   } else {
     // every wave needs every block: blocks pass through LDS, the next one on its way while one is at work
-    constexpr int EACH = 2 * KB * D * 2 / 1024 / NW;      // a wave's loads of a block
-    const auto fetch = [&](int b, int stage) __attribute__((always_inline)) {
-      const bool ring = b < RB;
-      const uint16_t* kb = ring ? ro.ring_k + b * (KB * D) : ro.k + (int64_t)(b - RB) * KB * p.nk_sl;
-      const uint16_t* vb = ring ? ro.ring_v + b * (KB * D) : ro.v + (int64_t)(b - RB) * KB * p.nv_sl;
-      const uint32_t to = lds_offset(&lds.stage[stage]) + 1024 * (EACH / 2) * wave;
-      // load e of the wave brings rows 2 o and 2 o + 1 of keys and values, o = wave * (EACH / 2) + e
-      const int l = lane_per_site(lane);
-      const int row = wave * EACH + (l >> 5);
-      const uint32_t k_piece = 16 * ((l & 31) ^ (row & 15)), v_piece = 16 * (l & 31);
-      // (the rows of a wave share all but bits 1 and 2, which 2 e sets)
-      if (whole >> b & 1u) {
-        const uint32_t k_off = row * (2 * D) + k_piece, v_off = row * (2 * D) + v_piece;
-#pragma unroll
-        for (int e = 0; e < EACH / 2; ++e) {
-          load_lds16(kb + 2 * e * D, k_off ^ (32 * e), to + 1024 * e);
-          load_lds16(vb + 2 * e * D, v_off, to + (uint32_t)offsetof(KeyStage, v) + 1024 * e);
-        }
-      } else {   // a key that no query sees is read as one that is
-        const uint32_t live = ring ? __builtin_amdgcn_readfirstlane(lds.live[b]) : live_nodes(b);
-        const uint32_t k_st = ring ? 2 * D : (uint32_t)(2 * p.nk_sl), v_st = ring ? 2 * D : (uint32_t)(2 * p.nv_sl);
-#pragma unroll
-        for (int e = 0; e < EACH / 2; ++e) {
-          const uint32_t at = live >> (row + 2 * e) & 1u ? (uint32_t)(row + 2 * e) : (uint32_t)__builtin_ctz(live);
-          load_lds16(kb, at * k_st + (k_piece ^ (32 * e)), to + 1024 * e);
-          load_lds16(vb, at * v_st + v_piece, to + (uint32_t)offsetof(KeyStage, v) + 1024 * e);
-        }
-      }
-    };
-    int stage = 0;
-    if (rest) fetch(__builtin_ctz(rest), 0);
-    while (rest) {
-      const int b = __builtin_ctz(rest);
+    int stage = 0, b = -1;
+    if (tree_first) b = RB, rest &= ~(1u << RB);
+    else if (rest) b = __builtin_ctz(rest), rest &= rest - 1, fetch(b, 0, whole >> b & 1u);
+    while (b >= 0) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // the block has landed
       __builtin_amdgcn_s_barrier();                       // for every wave; and the block before is read no more
       asm volatile("" ::: "memory");
+      const int next = rest ? __builtin_ctz(rest) : -1;
       rest &= rest - 1;
-      if (rest) fetch(__builtin_ctz(rest), stage ^ 1);
+      if (next >= 0) fetch(next, stage ^ 1, whole >> next & 1u);
       if (tiles > 0) {
         const KeyStage& ks_ = lds.stage[stage];
         const int c_here = lane_per_site(c);   // the addresses are made here rather than kept over the loop
@@ -534,15 +557,26 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
         }
         bf16x8 pb[T];
         softmax(b, S, pb);
+        // value operands by transpose reads: lane (g4, c) addresses key 4 g4 + c / 4, and of product i's dims 4 at 128 hh +
+        // 8 (4 q + i / 2) + 4 (i + q) % 2, q = c % 4; the products of two neighbours i read both halves of a piece
+        const int lane_here = lane_per_site(lane);
+        const int row = lane_here >> 2, q = lane_here & 3;
+        const uint16_t* const v_at = &ks_.v[row][8 * ((4 * q) ^ (row & 15)) + 4 * (q & 1)];
+        const uint32_t v_lds = lds_offset(v_at);
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          u32x4 vr[8];
+        for (int i = 0; i < 8; ++i) {
+          const uint16_t* const at = (const uint16_t*)(const __attribute__((address_space(3))) uint16_t*)(uintptr_t)(v_lds ^ (8 * i));
 #pragma unroll
-          for (int s = 0; s < 8; ++s)
-            vr[s] = *reinterpret_cast<const u32x4*>(&ks_.v[16 * (s >> 2) + 4 * g4 + (s & 3)][128 * hh + 8 * c]);
-          add_values(hh, vr, pb);
+          for (int hh = 0; hh < 2; ++hh) {
+            const u32x2 lo = ld_tr4(at + 128 * hh), hi = ld_tr4(at + 128 * hh + 16 * D);
+            const bf16x8 vf = as_bf16x8((u32x4){lo[0], lo[1], hi[0], hi[1]});
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+              O[t][hh][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pb[t], O[t][hh][i], 0, 0, 0);
+          }
         }
       }
+      b = next;
       stage ^= 1;
     }
   }
@@ -551,21 +585,21 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
   // (rows and addresses are made again here rather than kept over the loop)
   const int lane_end = lane_per_site(lane);
   const int ge = lane_end >> 4, ce = lane_end & 15;
-  // lane (ge, ce) of product (hh, i), register r: query ce, dim 128 hh + 32 ge + 8 r + i; a lane stores 8 R dims at a time
+  // lane (ge, ce) of product (hh, i), register r: query ce, dim 128 hh + 32 ge + 8 r + i, or (STAGED) + 8 (i / 2) + 4 ((i +
+  // ge) % 2) + r; a lane stores 8 R dims at a time
   constexpr int R = KW > 1 ? 8 / KW : 4;
   constexpr int TIMES = KW > 1 ? 1 : 2;
   const auto half_of = [&](int x) { return KW > 1 ? wk * R / 4 : x; };
   const int r0 = KW > 1 ? wk * R % 4 : 0;
-  // gates are loaded before the outputs that they could alias are stored: all of them, or (STAGED: registers) a tile's
-  u32x4 gw[STAGED ? 1 : T][TIMES][R];
-  const auto load_gates = [&](int t, int to) __attribute__((always_inline)) {
+  u32x4 gw[T][TIMES][R];
+  const auto load_gates = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < TIMES; ++x)
-      load_gate(p, ro, min(r_lo + 16 * t + ce, M - 1), 128 * half_of(x) + 32 * ge + 8 * r0, gw[to][x]);
+      load_gate(p, ro, min(r_lo + 16 * t + ce, M - 1), 128 * half_of(x) + 32 * ge + 8 * r0, gw[t][x]);
   };
-  if (!STAGED && p.splits == 1) {
+  if (p.splits == 1) {
 #pragma unroll
-    for (int t = 0; t < T; ++t) load_gates(t, t);
+    for (int t = 0; t < T; ++t) load_gates(t);
   }
 #pragma unroll
   for (int t = 0; t < T; ++t) sum[t] = add_xor32(add_xor16(sum[t]));
@@ -581,7 +615,6 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
 #pragma unroll
   for (int t = 0; t < T; ++t) {
     const int row = r_lo + 16 * t + ce;
-    if (STAGED && p.splits == 1) load_gates(t, 0);
     float top = m[t], total = sum[t];
     if constexpr (KW > 1) {
       top = -INFINITY;
@@ -618,7 +651,7 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y[8 * r + i] = O[t][x][i][r];
+          for (int r = 0; r < 4; ++r) y[4 * i + r] = ge & 1 ? O[t][x][i ^ 1][r] : O[t][x][i][r];
       }
       const int d0 = 128 * hh + 32 * ge + 8 * r0;
       if (row >= M) continue;
@@ -626,7 +659,7 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
         const float inv = 1.0f / total;
 #pragma unroll
         for (int e = 0; e < 8 * R; ++e) y[e] *= inv;
-        if (all_finite(y)) store_gated(p, ro, row, d0, y, gw[STAGED ? 0 : t][x]);
+        if (all_finite(y)) store_gated(p, ro, row, d0, y, gw[t][x]);
         else atomicOr(&lds.odd[wq * T + t], 1u << ce);
       } else {
         const int64_t at = ((int64_t)pair * p.splits + split) * ((int64_t)G * p.max_nodes) + row;
@@ -699,7 +732,7 @@ __global__ __launch_bounds__(256) void tree_attn_join_kernel(const TreeAttnParam
     unpack2(gate[0], gt[0], gt[1]);
     unpack2(gate[1], gt[2], gt[3]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] *= sigmoidf_(gt[e]);
+    for (int e = 0; e < 4; ++e) y[e] *= gate_of(gt[e]);
   }
   store4_bf16(ro.out + node * p.o_sl + g * p.o_sg + d0, y);
 }
