@@ -528,11 +528,12 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
     }
   } else {
     // every wave needs every block: blocks pass through LDS, the next one on its way while one is at work
+    constexpr int K_AHEAD = T == 1 ? 4 : 2, V_AHEAD = 5;   // pairs of reads
     int stage = 0, b = -1;
     if (tree_first) b = RB, rest &= ~(1u << RB);
     else if (rest) b = __builtin_ctz(rest), rest &= rest - 1, fetch(b, 0, whole >> b & 1u);
     while (b >= 0) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // the block has landed
+      __builtin_amdgcn_s_waitcnt(0x0f70);                 // vmcnt(0): the block has landed
       __builtin_amdgcn_s_barrier();                       // for every wave; and the block before is read no more
       asm volatile("" ::: "memory");
       const int next = rest ? __builtin_ctz(rest) : -1;
@@ -555,6 +556,15 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
             S[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qr[t][ks], S[t][1], 0, 0, 0);
           }
         }
+        // reads of the operands run ahead of the products
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * K_AHEAD, 0);
+#pragma unroll
+        for (int i = 0; i < D / 32 - K_AHEAD; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 2 * T, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * K_AHEAD * T, 0);
+        __builtin_amdgcn_sched_barrier(0);
         bf16x8 pb[T];
         softmax(b, S, pb);
         // value operands by transpose reads: lane (g4, c) addresses key 4 g4 + c / 4, and of product i's dims 4 at 128 hh +
@@ -575,6 +585,13 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
               O[t][hh][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pb[t], O[t][hh][i], 0, 0, 0);
           }
         }
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * V_AHEAD, 1);
+#pragma unroll
+        for (int i = 0; i < 16 - V_AHEAD; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, T, 1);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, V_AHEAD * T, 1);
       }
       b = next;
       stage ^= 1;
