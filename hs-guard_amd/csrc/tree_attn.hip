@@ -301,6 +301,7 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
   const uint64_t mask = threadIdx.x < MOST ? mask_of(ro.masks, min((int)threadIdx.x, len - 1)) : 0ull;
   bf16x8 qr[STAGED ? T : 1][D / 32];
   int node[T];
+  const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;    // a scale's sign goes to the queries
 #pragma unroll
   for (int t = 0; t < T; ++t) {
     const int row = min(r_lo + 16 * t + c, M - 1);           // past the valid rows: the last one again, not stored
@@ -309,12 +310,12 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
     node[t] = l;
     if constexpr (STAGED) {
 #pragma unroll
-      for (int ks = 0; ks < D / 32; ++ks) qr[t][ks] = as_bf16x8(load16(src + 32 * ks));
+      for (int ks = 0; ks < D / 32; ++ks) qr[t][ks] = as_bf16x8(load16(src + 32 * ks) ^ sign);
     } else {
       // the KW waves of the query group share the work
 #pragma unroll
       for (int ks = 0; ks < D / 32 / KW; ++ks)
-        lds.q[wq * T + t][wk * (D / 32 / KW) + ks][lane] = load16(src + 32 * (wk * (D / 32 / KW) + ks));
+        lds.q[wq * T + t][wk * (D / 32 / KW) + ks][lane] = load16(src + 32 * (wk * (D / 32 / KW) + ks)) ^ sign;
     }
   }
   const auto live_nodes = [&](int b) {   // of the tree's block b
@@ -405,12 +406,6 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
     const bool ring = b < RB;
     float top[T];
     bool move = false;
-    if (p.scale < 0.f) {
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) S[t][e >> 2][e & 3] = -S[t][e >> 2][e & 3];
-    }
     if (!(whole >> b & 1u)) {
       const int at = (ring ? b * KB : W_MAX + (b - RB) * KB) + 4 * g4;
       i32x4 place[2];
@@ -542,6 +537,8 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
       if (tiles > 0) {
         const KeyStage& ks_ = lds.stage[stage];
         const int c_here = lane_per_site(c);   // the addresses are made here rather than kept over the loop
+        // of two workgroups on a SIMD, the one at its products goes first (128 x 64 nodes 114 -> 109 us)
+        __builtin_amdgcn_s_setprio(1);
         f32x4 S[T][2];
 #pragma unroll
         for (int t = 0; t < T; ++t) S[t][0] = S[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -565,8 +562,10 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
         }
         __builtin_amdgcn_sched_group_barrier(0x008, 2 * K_AHEAD * T, 0);
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(0);
         bf16x8 pb[T];
         softmax(b, S, pb);
+        __builtin_amdgcn_s_setprio(1);
         // value operands by transpose reads: lane (g4, c) addresses key 4 g4 + c / 4, and of product i's dims 4 at 128 hh +
         // 8 (4 q + i / 2) + 4 (i + q) % 2, q = c % 4; the products of two neighbours i read both halves of a piece
         const int lane_here = lane_per_site(lane);
@@ -593,6 +592,7 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
         }
         __builtin_amdgcn_sched_group_barrier(0x008, V_AHEAD * T, 1);
       }
+      __builtin_amdgcn_s_setprio(0);
       b = next;
       stage ^= 1;
     }
