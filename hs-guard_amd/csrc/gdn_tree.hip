@@ -100,6 +100,11 @@ __device__ __forceinline__ uint32_t upper_pair(float a, float b) {
 }
 __device__ __forceinline__ float upper(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
+// silu to a few fp32 steps (its product is rounded to bf16): 5 instructions against siluf_'s 14, and a lane has up to 32
+__device__ __forceinline__ float silu_fast(float x) {
+  return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+}
+
 // Eight fp32 values as PARTS bf16 operands whose sum they are: 8 digits each, cut off rather than rounded
 template <int PARTS>
 __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&out)[PARTS]) {
@@ -369,13 +374,21 @@ __global__ __launch_bounds__(64 * NW, NT > 2 ? (HALF && NT == 3 ? 3 : 2) : HALF 
     const float kj = lds.kinv[j];
     const f32x4 be = *reinterpret_cast<const f32x4*>(&lds.beta[i0]), ki = *reinterpret_cast<const f32x4*>(&lds.kinv[i0]);
     const f32x4 qi = *reinterpret_cast<const f32x4*>(&lds.qinv[i0]);
+    float pv[4], av[4];
+    bool on[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = i0 + r;
-      const bool on = lds.mask[i] >> j & 1;
-      const float d = __builtin_amdgcn_exp2f((float)(lds.G[i] - Gj)) * kj;
-      lds.P[i][j] = on ? qi[r] * d * qk[e][r] : 0.f;
-      lds.A[i][j] = on && i != j ? -be[r] * ki[r] * d * kk[e][r] : 0.f;
+      on[r] = lds.mask[i0 + r] >> j & 1;
+      const float d = __builtin_amdgcn_exp2f((float)(lds.G[i0 + r] - Gj)) * kj;
+      pv[r] = qi[r] * d * qk[e][r];
+      av[r] = -be[r] * ki[r] * d * kk[e][r];
+      // made for every pair: a branch around each waits for its own reads (one tile: registers)
+      if constexpr (NT > 1) asm("" : "+v"(pv[r]), "+v"(av[r]));
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      lds.P[i0 + r][j] = on[r] ? pv[r] : 0.f;
+      lds.A[i0 + r][j] = on[r] && i0 + r != j ? av[r] : 0.f;
     }
   }
   lds_barrier();
@@ -502,7 +515,7 @@ __global__ __launch_bounds__(64 * NW, NT > 2 ? (HALF && NT == 3 ? 3 : 2) : HALF 
     for (int r = 0; r < 4; ++r) {
       const int i = 16 * t + 4 * g4 + r;
       const float o0 = o[t][0][r], o1 = o[t][1][r];
-      if (i < len) odd += (u[t][0][r] + u[t][1][r]) * 0.f + (o0 + o1) * 0.f;
+      odd += (u[t][0][r] + u[t][1][r]) * 0.f + (o0 + o1) * 0.f;   // (rows past the end: u is 0, o of the last row's q)
       if constexpr (GATED) {
         const float ss = sum16_dpp(o0 * o0 + o1 * o1);
         if (c == 0) lds.part[i][wave] = ss;
@@ -523,19 +536,25 @@ __global__ __launch_bounds__(64 * NW, NT > 2 ? (HALF && NT == 3 ? 3 : 2) : HALF 
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (t >= tiles) break;
+    uint32_t w[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * t + 4 * g4 + r;
       float y[2] = {o[t][0][r], o[t][1][r]};
       if constexpr (GATED) {
-        const f32x4 ss = *reinterpret_cast<const f32x4*>(lds.part[i]);
+        const f32x4 ss = *reinterpret_cast<const f32x4*>(lds.part[16 * t + 4 * g4 + r]);
         const float rs = rsqrtf(((ss[0] + ss[1]) + (ss[2] + ss[3])) * (1.0f / KD) + p.eps);
         float z[2];
         unpack2(zw[t][r], z[0], z[1]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) y[j] *= rs * w2[j] * siluf_(z[j]);
+        for (int j = 0; j < 2; ++j) y[j] *= rs * w2[j] * silu_fast(z[j]);
       }
-      if (i < len) *reinterpret_cast<uint32_t*>(ro.out + ((uint32_t)i * (uint32_t)(p.HV * KD) + col)) = pack_bf16x2(y[0], y[1]);
+      w[r] = pack_bf16x2(y[0], y[1]);
+      if constexpr (NT > 1) asm("" : "+v"(w[r]));   // made for every row: a branch around each waits for its own reads
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * t + 4 * g4 + r;
+      if (i < len) *reinterpret_cast<uint32_t*>(ro.out + ((uint32_t)i * (uint32_t)(p.HV * KD) + col)) = w[r];
     }
   }
 
