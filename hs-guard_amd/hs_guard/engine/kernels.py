@@ -418,12 +418,15 @@ def draft_tree_maps(parents, lens, starts, commits=None, max_nodes=HSG_TREE_MAX_
         raise AssertionError("parents must be [T]; lens, starts and commits [n]")
     if not 1 <= max_nodes <= HSG_TREE_MAX_NODES:
         raise AssertionError(f"max_nodes must be in [1, {HSG_TREE_MAX_NODES}]")
-    offsets, lens_out = torch.empty_like(lens), torch.empty_like(lens)
-    commits_out = None if commits is None else torch.empty_like(lens)
-    pos, masks = torch.empty_like(parents), torch.empty_like(parents)
-    _launch("hsg_tree_maps", device, parents.data_ptr(), parents.shape[0], lens.data_ptr(), starts.data_ptr(),
-            _ptr(commits), shape[0], max_nodes, offsets.data_ptr(), lens_out.data_ptr(), _ptr(commits_out), pos.data_ptr(),
-            masks.data_ptr())
+    n, total = shape[0], parents.shape[0]
+    # (one allocation for all: a small batch's cost is this function's own)
+    if commits is None:
+        commits_out = None
+        offsets, lens_out, pos, masks = parents.new_empty(2 * (n + total)).split((n, n, total, total))
+    else:
+        offsets, lens_out, commits_out, pos, masks = parents.new_empty(3 * n + 2 * total).split((n, n, n, total, total))
+    _launch("hsg_tree_maps", device, parents.data_ptr(), total, lens.data_ptr(), starts.data_ptr(), _ptr(commits), n,
+            max_nodes, offsets.data_ptr(), lens_out.data_ptr(), _ptr(commits_out), pos.data_ptr(), masks.data_ptr())
     return DraftTrees(offsets, lens_out, commits_out, pos, masks, max_nodes)
 
 
