@@ -4,25 +4,27 @@
 // tree's keys those of its ancestors and its own that lie within W of it. Nothing of the ring moves but, in a second launch
 // after all reads, the columns of the committed chain.
 //
-// Query rows r = node * G + (query head of the kv head) form tiles of 16, 1 or 2 to a wave. Per block of 32 keys, on
+// Query rows r = node * G + (query head of the kv head) form tiles of 16, one or two to a wave. Per block of 32 keys, on
 // v_mfma_f32_16x16x32_bf16:
 //   S^T[key, query] = K . Q^T      a lane's column is one query: maxima, sums and rescales are per-lane scalars
-//   O^T[d, query] += V^T . P^T     B = P straight from the S^T accumulators (the product's key order is the lane's own);
-//                                  A = V^T: a lane reads 8 dims of its 8 keys and swaps 16-bit halves in registers, product
-//                                  i of 8 taking dim 8 c + i of each lane c
+//   O^T[d, query] += V^T . P^T     B = P straight from the S^T accumulators (the product's key order is the lane's own)
 // The running maximum is moved only when a block's exceeds it by 2^8, so the accumulators are seldom rescaled; sums are fp32
-// and P is rounded to bf16 for its product (2^-9 of each weight, below the output's own rounding).
+// and P is rounded to bf16 for its product (2^-9 of each weight, below the output's own rounding), the weights' sum taking it
+// as rounded.
 //
-// Up to 64 query rows a (row, kv head), bound by reading the ring: the waves of a query group split its KEYS, a wave's keys
-// and values going straight from memory to its operand registers (2 tiles a wave: 380 registers), and meet in LDS at the end,
-// weighted by their maxima; no barrier and no LDS write in the loop. 352 rows of one node over full rings, 16 q / 4 kv heads:
-// 129 us, 5.1 TB/s.
-// More query rows, bound by the products: every wave has 32 rows of its own and needs every key, so blocks pass through LDS
-// once for the four waves (128 KB: three blocks ahead, direct-to-LDS loads counted by vmcnt, one barrier a block). 128 rows of
-// 64 nodes 224 us. With 4 tiles a wave instead, from registers, the accumulators alone took half of them and the spills made
-// it 1,040 us.
+// Up to 16 query rows a (row, kv head), bound by reading the ring: the four waves split its KEYS, a wave's keys and values going
+// straight from memory to its operand registers (of a value 8 dims of a lane's 8 keys, whose 16-bit halves it swaps), and meet
+// in LDS at the end, weighted by their maxima; no barrier and no LDS write in the loop. 352 rows of one node over full rings, 16
+// q / 4 kv heads: 120 us, 5.5 TB/s.
+// More query rows: every wave has one or two tiles of its own and needs every key, so blocks pass through LDS once for the four
+// waves (two stages of 32 KB, direct-to-LDS loads, one barrier a block; two workgroups on a CU). Keys are read as they lie,
+// values by transpose reads, both ahead of their products, and waves at their products go before waves at their softmax. 128
+// rows of 64 nodes: 109 us, where the bytes alone take 78; a block of a workgroup takes 2.1 us, of which its 64 products a wave
+// are 0.9 for the two workgroups that share a SIMD, the rest softmax, LDS reads and the issue of the next block's loads; 5.5 us
+// before the loop (ring positions, queries, first block) and 6 after it (gates, outputs) are not hidden. Operands by byte
+// permutes instead of transpose reads and reads right before their products made it 131 us; four tiles a wave spilled: 1,040 us.
 // Where few rows leave the chip short of workgroups, workgroups split a row's key blocks further and a second launch joins
-// their partial sums: a lone row of 12 nodes 12.7 + 8.6 us.
+// their partial sums: a lone row of 12 nodes 9.4 + 3.7 us, both a chain of dependent loads.
 //
 // A masked pair has P = 0, which would carry a NaN or an infinity of a value to queries that do not see it: columns that no
 // query of the row sees are not read (another key's are, in their place), and a query row with a result that is not finite is
@@ -242,16 +244,14 @@ struct KeyStage {
   uint16_t v[KB][D];
 };
 
-template <int T, int KW, bool STAGED>
+// T: tiles of a wave; STAGED: keys pass through LDS, else the waves split them
+template <int T, bool STAGED>
 struct TreeAttnLds {
-  static constexpr int QW = NW / KW;
-  static constexpr int STAGES = STAGED ? 2 : 1;
+  static constexpr int QW = STAGED ? NW : 1;    // waves with queries of their own
   union {
-    struct {
-      u32x4 q[STAGED ? 1 : QW * T][D / 32][64];   // the queries' operands, in the order of the lanes
-    };
-    KeyStage stage[STAGES];
-    f32x4 o[KW > 1 ? NW : 1][16][64];             // a tile's partial sums of every wave
+    u32x4 q[STAGED ? 1 : D / 32][64];           // the queries' operands, in the order of the lanes
+    KeyStage stage[STAGED ? 2 : 1];
+    f32x4 o[STAGED ? 1 : NW][16][64];           // every wave's partial sums
   };
   int kp[W_MAX + MOST];       // places of the ring's keys before the start; then the nodes' depths
   uint64_t mask[MOST];        // the nodes' ancestors and themselves
@@ -262,11 +262,12 @@ struct TreeAttnLds {
   __device__ TreeAttnLds() {}
 };
 
-template <int T, int KW, bool STAGED>
-__global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_kernel(const TreeAttnParams p) {
-  constexpr int QW = NW / KW;
+template <int T, bool STAGED>
+__global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(const TreeAttnParams p) {
+  static_assert(STAGED || T == 1, "the split of the keys takes one tile");
+  constexpr int QW = STAGED ? NW : 1, KW = NW / QW;   // waves of queries, of keys
   constexpr int ROWS = 16 * T * QW;     // query rows of the workgroup
-  __shared__ __align__(16) TreeAttnLds<T, KW, STAGED> lds;
+  __shared__ __align__(16) TreeAttnLds<T, STAGED> lds;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wk = wave % KW, wq = wave / KW;
@@ -312,10 +313,8 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
 #pragma unroll
       for (int ks = 0; ks < D / 32; ++ks) qr[t][ks] = as_bf16x8(load16(src + 32 * ks) ^ sign);
     } else {
-      // the KW waves of the query group share the work
 #pragma unroll
-      for (int ks = 0; ks < D / 32 / KW; ++ks)
-        lds.q[wq * T + t][wk * (D / 32 / KW) + ks][lane] = load16(src + 32 * (wk * (D / 32 / KW) + ks)) ^ sign;
+      for (int ks = wk; ks < D / 32; ks += KW) lds.q[ks][lane] = load16(src + 32 * ks) ^ sign;
     }
   }
   const auto live_nodes = [&](int b) {   // of the tree's block b
@@ -399,7 +398,6 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
     const uint32_t some = (uint32_t)__ballot(lane < RB && lds.live[min(lane, BLOCKS - 1)] != 0u) | (~0u << RB);
     whole = (uint32_t)__ballot(lane < RB && lds.whole[min(lane, BLOCKS - 1)] != 0u);
     for (int b = b_first; b < n_blocks; b += step) rest |= some & (1u << b);
-    if (tiles == 0 && KW > 1) rest = 0u;
   }
   // probabilities of block b for the scores S, rounded; the accumulators follow a maximum that has moved
   const auto softmax = [&](int b, f32x4 (&S)[T][2], bf16x8 (&pb)[T]) __attribute__((always_inline)) {
@@ -509,7 +507,7 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
       for (int ks = 0; ks < D / 32; ++ks)
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-          const bf16x8 qf = as_bf16x8(lds.q[wq * T + t][ks][lane]);
+          const bf16x8 qf = as_bf16x8(lds.q[ks][lane]);
           S[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[0][ks]), qf, S[t][0], 0, 0, 0);
           S[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kr[1][ks]), qf, S[t][1], 0, 0, 0);
         }
@@ -604,10 +602,9 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
   const int ge = lane_end >> 4, ce = lane_end & 15;
   // lane (ge, ce) of product (hh, i), register r: query ce, dim 128 hh + 32 ge + 8 r + i, or (STAGED) + 8 (i / 2) + 4 ((i +
   // ge) % 2) + r; a lane stores 8 R dims at a time
-  constexpr int R = KW > 1 ? 8 / KW : 4;
-  constexpr int TIMES = KW > 1 ? 1 : 2;
-  const auto half_of = [&](int x) { return KW > 1 ? wk * R / 4 : x; };
-  const int r0 = KW > 1 ? wk * R % 4 : 0;
+  constexpr int R = STAGED ? 4 : 8 / KW, TIMES = STAGED ? 2 : 1;
+  const auto half_of = [&](int x) { return STAGED ? x : wk * R / 4; };
+  const int r0 = STAGED ? 0 : wk * R % 4;
   u32x4 gw[T][TIMES][R];
   const auto load_gates = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
@@ -620,7 +617,7 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
   }
 #pragma unroll
   for (int t = 0; t < T; ++t) sum[t] = add_xor32(add_xor16(sum[t]));
-  if constexpr (KW > 1) {
+  if constexpr (!STAGED) {
 #pragma unroll
     for (int t = 0; t < T; ++t)
       if (ge == 0) {
@@ -633,16 +630,15 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
   for (int t = 0; t < T; ++t) {
     const int row = r_lo + 16 * t + ce;
     float top = m[t], total = sum[t];
-    if constexpr (KW > 1) {
+    if constexpr (!STAGED) {
       top = -INFINITY;
       total = 0.f;
 #pragma unroll
-      for (int w = 0; w < KW; ++w) top = fmaxf(top, lds.ml[wq * KW + w][t][ce][0]);
+      for (int w = 0; w < KW; ++w) top = fmaxf(top, lds.ml[w][t][ce][0]);
       const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-      for (int w = 0; w < KW; ++w) total += exp2_fast(lds.ml[wq * KW + w][t][ce][0] - base) * lds.ml[wq * KW + w][t][ce][1];
+      for (int w = 0; w < KW; ++w) total += exp2_fast(lds.ml[w][t][ce][0] - base) * lds.ml[w][t][ce][1];
       const float mine = exp2_fast(m[t] - base);
-      if (t) __syncthreads();   // the tile before is read
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
@@ -653,14 +649,14 @@ __global__ __launch_bounds__(64 * NW, T == 1 || STAGED ? 2 : 1) void tree_attn_k
     for (int x = 0; x < TIMES; ++x) {
       const int hh = half_of(x);
       float y[8 * R];
-      if constexpr (KW > 1) {
+      if constexpr (!STAGED) {
 #pragma unroll
         for (int e = 0; e < 8 * R; ++e) y[e] = 0.f;
 #pragma unroll
         for (int w = 0; w < KW; ++w)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float* src = reinterpret_cast<const float*>(&lds.o[wq * KW + w][8 * hh + i][lane_end]) + r0;
+            const float* src = reinterpret_cast<const float*>(&lds.o[w][8 * hh + i][lane_end]) + r0;
 #pragma unroll
             for (int r = 0; r < R; ++r) y[8 * r + i] += src[r];
           }
@@ -784,22 +780,22 @@ __global__ __launch_bounds__(256) void tree_ring_write_kernel(const TreeAttnPara
   }
 }
 
-// Query rows of a workgroup. Up to 16 the waves split their keys (352 x 1 node 124 us, against 140 through LDS); beyond, keys
-// pass through LDS for 4 waves of one tile, or of two where that fills the chip (256 CUs) and wastes little: a workgroup of
-// 128 rows takes 1.5 times as long as one of 64. 64 x 64 nodes, 16 q / 4 kv heads: 68 us with 128 rows, 88 with 64; 20 x 64
-// 44 and 38; 100 x 33 (129 to 192 rows are three workgroups of 64) 109 and 86.
+// Query rows of a workgroup. Up to 16 the waves split their keys (352 x 1 node 122 us, against 127 through LDS); beyond, keys
+// pass through LDS for 4 waves of one tile, or of two where that fills the chip (256 CUs) and wastes little. 64 x 64 nodes, 16 q
+// / 4 kv heads: 55 us with 128 rows, 68 with 64; 20 x 64 36 and 30; 100 x 33 (129 to 192 rows are three workgroups of 64) 84 and
+// 67.
 inline int rows_of(int64_t pairs, int64_t rows) {
   if (rows <= 64) return rows <= 16 ? 16 : 64;
   return (rows + 63) / 64 == 3 || pairs * ((rows + 127) / 128) < 256 ? 64 : 128;
 }
 
-// Workgroups of a row's key blocks: few rows leave the chip short of workgroups, and one CU moves only a few tens of GB/s.
-// Twice as many for twice as many units were no faster: 30 x 14 nodes (120 units) 21 us with 2 and with 4, 60 x 14 42 us with 1
-// against 33 and a join of 12 with 2.
+// Workgroups of a row's key blocks: few rows leave the chip short of workgroups, and one CU moves only a few tens of GB/s. 16 x 4
+// nodes (64 units): 14.0, 12.5 and 13.4 us with 2, 4 and 8, and a join of 3.9; 30 x 14 (120): 24.7 with 1, as long as 18.0 with 2
+// and a join of 6.6; 60 x 14 32.4 with 1, 28.9 and 11.7 with 2.
 inline int splits_of(int64_t pairs, int64_t rows) {
   const int per = rows_of(pairs, rows);
   const int64_t units = pairs * ((rows + per - 1) / per);
-  return units <= 32 ? SPLITS_MAX : units <= 64 ? 4 : units <= 128 ? 2 : 1;
+  return units <= 32 ? SPLITS_MAX : units <= 64 ? 4 : 1;
 }
 
 inline size_t part_bytes(int64_t pairs, int64_t rows, int splits) {
@@ -868,9 +864,9 @@ extern "C" int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int
   if (blocks >= (1 << 24)) return HSG_ERR_SHAPE;   // a launch holds less than 2^32 threads
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * NW), 0, st, p); };
-  if (per_wg == 16) launch(tree_attn_kernel<1, 4, false>);
-  else if (per_wg == 64) launch(tree_attn_kernel<1, 1, true>);
-  else launch(tree_attn_kernel<2, 1, true>);
+  if (per_wg == 16) launch(tree_attn_kernel<1, false>);
+  else if (per_wg == 64) launch(tree_attn_kernel<1, true>);
+  else launch(tree_attn_kernel<2, true>);
   if (p.splits > 1)
     hipLaunchKernelGGL(tree_attn_join_kernel, dim3((unsigned)pairs, (unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
   if (commits)

@@ -329,7 +329,7 @@ def test_attention(lens, hkv, G, W, commit, gated):
 
 @pytest.mark.parametrize("rows_n", [1, 20, 300])
 def test_attention_over_many_rows(rows_n):
-    """Every way a call splits its keys (4, 2 and 1 workgroups a row), at head counts of the released model."""
+    """Every way a call splits its keys (8, 4 and 1 workgroups a row), at head counts of the released model."""
     rng = np.random.default_rng(rows_n)
     lens = rng.integers(1, 9 if rows_n > 100 else 20, rows_n).tolist()
     hkv, G, W = 2, 4, 512
