@@ -526,6 +526,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(const TreeAttnPar
     if (tree_first) b = RB, rest &= ~(1u << RB);
     else if (rest) b = __builtin_ctz(rest), rest &= rest - 1, fetch(b, 0, whole >> b & 1u);
     while (b >= 0) {
+      asm volatile("" ::: "memory");                      // the block before has been read
       __builtin_amdgcn_s_waitcnt(0x0f70);                 // vmcnt(0): the block has landed
       __builtin_amdgcn_s_barrier();                       // for every wave; and the block before is read no more
       asm volatile("" ::: "memory");

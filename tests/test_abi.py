@@ -195,32 +195,35 @@ def test_tree_operators_refuse_before_launch():
         assert conv(**bad) == rc, bad
 
     def step(*, qkv=256, stride=512, a=256, state=256, dtype=0, state_rows=2, masks=256, rows=2, most=64, H=1, HV=1, K=128,
-             V=128, z=256, z_stride=128, norm=256, out=512, off=0, ab=1):
+             V=128, scale=1.0, z=256, z_stride=128, norm=256, out=512, off=0, ab=1):
         return L.hsg_gdn_tree_step(qkv, stride, off, 128, 256, a, 256, ab, 256, 256, state, dtype, state_rows, 256, 256,
-                                   256, None, masks, rows, most, H, HV, K, V, 1.0, z, z_stride, norm, 1e-6, out, None)
+                                   256, None, masks, rows, most, H, HV, K, V, scale, z, z_stride, norm, 1e-6, out, None)
 
     assert step(rows=0) == 0
     for bad, rc in (({"K": 64}, SHAPE), ({"V": 64}, SHAPE), ({"most": 65}, SHAPE), ({"rows": 1 << 24}, SHAPE),
                     ({"HV": 3, "H": 2}, ARG), ({"dtype": 2}, ARG), ({"a": None}, ARG), ({"masks": None}, ARG),
                     ({"norm": None}, ARG), ({"z_stride": 64}, ARG), ({"ab": 0}, ARG), ({"off": -8}, ARG),
                     ({"state_rows": 0}, ARG), ({"stride": 516}, ALIGN), ({"off": 4}, ALIGN), ({"state": 264}, ALIGN),
-                    ({"z": 258}, ALIGN), ({"out": 514}, ALIGN)):
+                    ({"z": 258}, ALIGN), ({"out": 514}, ALIGN), ({"scale": float("inf")}, ARG),
+                    ({"stride": 1 << 24}, SHAPE), ({"z_stride": 1 << 24}, SHAPE)):
         assert step(**bad) == rc, bad
 
-    def attend(*, q=256, q_sl=512, ring_k=256, ring_rows=2, window=512, k_sl=256, gate=256, g_sl=1024, ring_pos=256,
-               masks=256, rows=2, most=64, hkv=1, G=2, dim=256, out=512, o_sl=512, ws=None, ws_bytes=0):
-        return L.hsg_tree_attention(q, q_sl, 512, 256, ring_k, 256, ring_rows, window, 256, k_sl, 256, 256, 256, 256, gate,
+    def attend(*, q=256, q_sl=512, ring_k=256, ring_rows=2, window=512, k_sl=256, v_sl=256, scale=1.0, gate=256,
+               g_sl=1024, ring_pos=256, masks=256, rows=2, most=64, hkv=1, G=2, dim=256, out=512, o_sl=512, ws=None,
+               ws_bytes=0):
+        return L.hsg_tree_attention(q, q_sl, 512, 256, ring_k, 256, ring_rows, window, 256, k_sl, 256, 256, v_sl, 256, gate,
                                     g_sl, 1024, 512, 256, ring_pos, 256, 256, 256, 256, None, masks, rows, most, hkv, G,
-                                    dim, 1.0, out, o_sl, 512, 256, ws, ws_bytes, None)
+                                    dim, scale, out, o_sl, 512, 256, ws, ws_bytes, None)
 
     assert attend(rows=0) == 0
     for bad, rc in (({"dim": 128}, SHAPE), ({"window": 544}, SHAPE), ({"window": 40}, SHAPE), ({"most": 65}, SHAPE),
                     ({"rows": 1 << 24}, SHAPE), ({"hkv": 0}, ARG), ({"G": 0}, ARG), ({"ring_rows": 0}, ARG),
                     ({"q": None}, ARG), ({"ring_pos": None}, ARG), ({"masks": None}, ARG), ({"q_sl": 516}, ALIGN),
                     ({"k_sl": 260}, ALIGN), ({"g_sl": 1028}, ALIGN), ({"q": 264}, ALIGN), ({"out": 520}, ALIGN),
-                    ({"ws": 264, "ws_bytes": 1 << 30}, ALIGN)):
+                    ({"ws": 264, "ws_bytes": 1 << 30}, ALIGN), ({"scale": float("nan")}, ARG),
+                    ({"k_sl": 1 << 24}, SHAPE), ({"v_sl": -256}, SHAPE)):
         assert attend(**bad) == rc, bad
     need = L.hsg_tree_attention_workspace_bytes
     assert need(1, 4, 4, 12) == 4 * 8 * 48 * 258 * 4      # 4 kv heads, 8 splits, 48 query rows of 256 sums, maximum, weight
-    assert need(20, 4, 4, 12) == 20 * 4 * 2 * 48 * 258 * 4
+    assert need(12, 4, 4, 12) == 12 * 4 * 4 * 48 * 258 * 4 and need(20, 4, 4, 12) == 0
     assert need(352, 4, 4, 12) == 0 and need(0, 4, 4, 12) == 0 and need(1, 4, 4, 65) == 0
