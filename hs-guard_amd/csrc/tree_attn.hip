@@ -19,7 +19,7 @@
 // More query rows: every wave has one or two tiles of its own and needs every key, so blocks pass through LDS once for the four
 // waves (two stages of 32 KB, direct-to-LDS loads, one barrier a block; two workgroups on a CU). Keys are read as they lie,
 // values by transpose reads, both ahead of their products, and waves at their products go before waves at their softmax. 128
-// rows of 64 nodes: 109 us, where the bytes alone take 78; a block of a workgroup takes 2.1 us, of which its 64 products a wave
+// rows of 64 nodes with commits: 109 us, where the bytes alone take 78; a block of a workgroup takes 2.1 us, of which its 64 products a wave
 // are 0.9 for the two workgroups that share a SIMD, the rest softmax, LDS reads and the issue of the next block's loads; 5.5 us
 // before the loop (ring positions, queries, first block) and 6 after it (gates, outputs) are not hidden. Operands by byte
 // permutes instead of transpose reads and reads right before their products made it 131 us; four tiles a wave spilled: 1,040 us.
