@@ -1,8 +1,8 @@
 // Window attention of a drafted tree's nodes over the slot's ring and each node's own ancestors, gated, for gfx950 on MFMA.
 //
 // Node i of a row stands at start + depth_i. It sees the ring's keys at 0 <= p < start, p > start + depth_i - W, and of the
-// tree's keys those of its ancestors and its own that lie within W of it. Nothing of the ring moves but, in a second launch
-// after all reads, the columns of the committed chain.
+// tree's keys those of its ancestors and its own that lie within W of it. Nothing of the ring moves but the columns of the
+// committed chain, after all reads: at its workgroup's end where a (row, kv head) has one, else in a launch of its own.
 //
 // Query rows r = node * G + (query head of the kv head) form tiles of 16, one or two to a wave. Per block of 32 keys, on
 // v_mfma_f32_16x16x32_bf16:
@@ -66,6 +66,7 @@ struct TreeAttnParams {
   int pairs;        // rows x kv heads
   int qblocks;      // workgroups of query rows a pair
   int splits;       // workgroups of key blocks
+  bool write_here;  // rows commit, and a pair has one workgroup
   float* part_o;    // [pair][split][query row][D]: partial sums
   float* part_ml;   // [pair][split][query row][2]: their maxima and weights' sums
   uint16_t* out; int64_t o_sl, o_sh, o_sg;
@@ -215,6 +216,36 @@ __device__ __forceinline__ void store_gated(const TreeAttnParams& p, const TreeK
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(y[e + 2 * i], y[e + 2 * i + 1]);
     *reinterpret_cast<u32x4*>(dst + e) = w;
+  }
+}
+
+// The committed chain's keys and values into the ring (of a chain longer than the window its last W), 16 nodes at a time of
+// which the caller takes every `step`-th: a thread's 16-byte pieces are loaded before any of them is stored
+__device__ __forceinline__ void write_chain(const TreeAttnParams& p, int n, int h, int block, int step) {
+  const int64_t slot = p.slots[n], len = p.lens[n], off = p.offsets[n], start = p.starts[n], done64 = p.commits[n];
+  if ((slot < 0) | (slot >= p.ring_rows) | (len <= 0) | (len > p.max_nodes) | (done64 <= 0)) return;
+  const int done = (int)(done64 > len ? len : done64);
+  const int64_t ring = ((slot * p.hkv + h) * (int64_t)(p.W + 1)) * D;
+  const int64_t start_col = ((start % p.W) + p.W) % p.W;
+  constexpr int EACH = 2;   // nodes of a thread: 8 nodes of 32 pieces at a time
+  const int d = 8 * (threadIdx.x & 31);
+  for (int first = max(0, done - p.W) + block * (8 * EACH); first < done; first += step * (8 * EACH)) {
+    u32x4 k[EACH], v[EACH];
+    int node[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      node[e] = first + 8 * e + (int)(threadIdx.x >> 5);
+      const int64_t t = off + min(node[e], done - 1);
+      k[e] = load16(p.new_k + t * p.nk_sl + h * p.nk_sh + d);
+      v[e] = load16(p.new_v + t * p.nv_sl + h * p.nv_sh + d);
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      if (node[e] >= done) continue;
+      const int64_t at = ring + ((start_col + node[e]) % p.W) * D + d;
+      *reinterpret_cast<u32x4*>(p.ring_k + at) = k[e];
+      *reinterpret_cast<u32x4*>(p.ring_v + at) = v[e];
+    }
   }
 }
 
@@ -699,6 +730,16 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(const TreeAttnPar
       walk_keys(p, ro, r_wg + i, d0, y);
       store_gated(p, ro, r_wg + i, d0, y, one);
     }
+  // ---- the pair's only workgroup writes its committed chain after its reads: 64 x 12 nodes 35.6 us, with a launch for it 34.2 +
+  // 4.1; 352 x 1 125.8 and 122.4 + 4.8. (The arguments are loaded again: kept over the loop, they took the scalar registers that
+  // its schedule needs.) ----
+  const auto* args = (const __attribute__((address_space(4))) TreeAttnParams*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  const TreeAttnParams& late = *(const TreeAttnParams*)args;
+  if (late.write_here) {
+    __syncthreads();
+    write_chain(late, (int)blockIdx.x / late.hkv, (int)blockIdx.x % late.hkv, 0, 1);
+  }
 }
 
 // Joins the splits' partial sums: a wave a query row, 4 dims a lane; every split's loads are in flight at once
@@ -751,34 +792,8 @@ __global__ __launch_bounds__(256) void tree_attn_join_kernel(const TreeAttnParam
   store4_bf16(ro.out + node * p.o_sl + g * p.o_sg + d0, y);
 }
 
-// The committed chain's keys and values into the ring (of a chain longer than the window its last W), 16 nodes a workgroup:
-// a thread's 16-byte pieces are loaded before any of them is stored
 __global__ __launch_bounds__(256) void tree_ring_write_kernel(const TreeAttnParams p) {
-  const int n = blockIdx.x / p.hkv, h = blockIdx.x - n * p.hkv;
-  const int64_t slot = p.slots[n], len = p.lens[n], off = p.offsets[n], start = p.starts[n], done64 = p.commits[n];
-  if ((slot < 0) | (slot >= p.ring_rows) | (len <= 0) | (len > p.max_nodes) | (done64 <= 0)) return;
-  const int done = (int)(done64 > len ? len : done64);
-  const int first = max(0, done - p.W);
-  const int64_t ring = ((slot * p.hkv + h) * (int64_t)(p.W + 1)) * D;
-  const int64_t start_col = ((start % p.W) + p.W) % p.W;
-  constexpr int EACH = 2;   // nodes of a thread: 8 nodes of 32 pieces at a time
-  const int d = 8 * (threadIdx.x & 31);
-  u32x4 k[EACH], v[EACH];
-  int node[EACH];
-#pragma unroll
-  for (int e = 0; e < EACH; ++e) {
-    node[e] = first + blockIdx.y * (8 * EACH) + 8 * e + (int)(threadIdx.x >> 5);
-    const int64_t t = off + min(node[e], done - 1);
-    k[e] = load16(p.new_k + t * p.nk_sl + h * p.nk_sh + d);
-    v[e] = load16(p.new_v + t * p.nv_sl + h * p.nv_sh + d);
-  }
-#pragma unroll
-  for (int e = 0; e < EACH; ++e) {
-    if (node[e] >= done) continue;
-    const int64_t at = ring + ((start_col + node[e]) % p.W) * D + d;
-    *reinterpret_cast<u32x4*>(p.ring_k + at) = k[e];
-    *reinterpret_cast<u32x4*>(p.ring_v + at) = v[e];
-  }
+  write_chain(p, blockIdx.x / p.hkv, blockIdx.x % p.hkv, blockIdx.y, gridDim.y);
 }
 
 // Query rows of a workgroup. Up to 16 the waves split their keys (352 x 1 node 122 us, against 127 through LDS); beyond, keys
@@ -858,6 +873,7 @@ extern "C" int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int
   p.qblocks = (int)((rows + per_wg - 1) / per_wg);
   p.splits = splits_of(pairs, rows);
   if (!workspace || workspace_bytes < part_bytes(pairs, rows, p.splits)) p.splits = 1;
+  p.write_here = commits && p.qblocks == 1 && p.splits == 1;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.splits > 1 ? p.part_o + pairs * p.splits * rows * D : nullptr;
   p.out = static_cast<uint16_t*>(out); p.o_sl = o_sl; p.o_sh = o_sh; p.o_sg = o_sg;
@@ -870,7 +886,7 @@ extern "C" int hsg_tree_attention(const void* q, int64_t q_sl, int64_t q_sh, int
   else launch(tree_attn_kernel<2, true>);
   if (p.splits > 1)
     hipLaunchKernelGGL(tree_attn_join_kernel, dim3((unsigned)pairs, (unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
-  if (commits)
+  if (commits && !p.write_here)
     hipLaunchKernelGGL(tree_ring_write_kernel, dim3((unsigned)pairs, (unsigned)((max_nodes + 15) / 16)), dim3(256), 0, st, p);
   return launch_status();
 }

@@ -577,7 +577,7 @@ int hsg_gdn_tree_step(const void* qkv, int64_t qkv_stride, int32_t q_off, int32_
  * position - window < theirs. out = bf16(softmax(scale q.k) . v * sigmoid(gate)), rounded once; probabilities are rounded to
  * bf16 for their product. gate may be NULL: no gating. Element addresses, ring pools and ring_pos as hsg_ring_attention's
  * packed layout. Rows with commits[n] > 0 write their chain's keys and values into the ring columns (starts[n] + j) % window
- * (of a chain longer than the window the last `window`), in a launch after the reads; ring_pos is the caller's
+ * (of a chain longer than the window the last `window`), after all reads of them; ring_pos is the caller's
  * (hsg_ring_pos_update with lens = commits). A NaN or an infinity reaches only the nodes that see it. out must not overlap
  * an input.
  * workspace (optional): with at least hsg_tree_attention_workspace_bytes(n_rows, hkv, groups, max_nodes) bytes (0: none is
