@@ -272,6 +272,27 @@ def test_gdn_keeps_a_bad_node_to_its_branch(what, n):
         assert torch.equal(state[[0, 2]], s["state"][[0, 2]])
 
 
+@pytest.mark.parametrize("n", [12, 24, 40])
+def test_gdn_recomputed_rows_of_an_fp16_state(n):
+    """One value of the last node of one row of three is not finite: all else, and every state, as without it."""
+    H, HV = 1, 2
+    parents = [-1, 0] + [0] * (n - 2)
+    rows, slots, _, pool_rows, dev = batch(6, [n] * 3, True)
+    rows = [(r * n, parents, 2) for r in range(3)]
+    dev["parents"] = torch.tensor(parents * 3, device="cuda")
+    dev["commits"] = torch.tensor([2] * 3, device="cuda")
+    s = gdn_inputs(n, 3 * n, pool_rows, H, HV, torch.float16)
+    o, osize, st, ssize = gdn_oracle(s, H, HV, slots, rows)
+    y, ysize = tree.gated(o, osize, _f64(s["z"]).reshape(o.shape), _f64(s["norm_weight"]), 1e-6)
+    s["packed"][2 * n - 1, 2 * H * KD + 7] = float("nan")
+    state = s["state"].clone()
+    out = gdn_call(s, H, HV, dev["slots"], maps_of(dev, n), state).reshape(o.shape)
+    rest = [i for i in range(3 * n) if i != 2 * n - 1]
+    within(out[rest], y[rest], 2.0 ** -15 * ysize[rest], 2.0 ** -8, "the other nodes")
+    within(state, st, 2.0 ** -15 * ssize, 2.0 ** -11, "state")
+    assert not torch.isfinite(out[2 * n - 1, 0]).any() and torch.isfinite(out[2 * n - 1, 1]).all()
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------------------------------------------
@@ -392,6 +413,75 @@ def test_attention_keeps_a_bad_value_to_who_sees_it(n, G, value):
                 keep = [d for d in range(G * D) if d % D != 5]
                 within(out[below][:, keep], want[below][:, keep], slack[below][:, keep], 2.0 ** -8, "its other dims")
     assert rest
+
+
+@pytest.mark.parametrize("rows_n,n,G,W", [(70, 3, 4, 512), (70, 12, 4, 64), (70, 40, 4, 64), (260, 64, 2, 32)])
+def test_attention_of_many_rows_with_bad_values(rows_n, n, G, W):
+    """As many rows as leave none split: one workgroup a row (which writes its committed chain itself) or several. A value of
+    three rows' last node is not finite: only these nodes see it, and the rings take it where it is committed."""
+    hkv, bad = 1, (0, 7, rows_n - 1)
+    parents = [-1, 0] + [(i - 1) // 2 for i in range(2, n)]
+    total = rows_n * n
+    rng = np.random.default_rng(rows_n + n)
+    slots = rng.permutation(rows_n + 1)[:rows_n].tolist()
+    starts = rng.integers(0, 3 * W, rows_n).tolist()
+    commits = [2 if r % 3 else 0 for r in range(rows_n)]
+    dev = {"parents": torch.tensor(parents * rows_n, device="cuda"), "lens": torch.tensor([n] * rows_n, device="cuda"),
+           "starts": torch.tensor(starts, device="cuda"), "commits": torch.tensor(commits, device="cuda"),
+           "slots": torch.tensor(slots, device="cuda")}
+    s = attention_inputs(n, total, rows_n + 1, slots, starts, hkv, G, W)
+    some = sorted({*bad, 1, 2, rows_n // 2})
+    rows = [(r * n, parents, commits[r]) for r in range(rows_n)]
+    want, slack, _, _ = attention_oracle(s, [slots[r] for r in some], [starts[r] for r in some], [rows[r] for r in some], W,
+                                         0.0625)
+    rings = s["ring_k"].clone(), s["ring_v"].clone()
+    clean = attention_call(s, dev, maps_of(dev, n), W, 0.0625, rings)
+    last = [r * n + n - 1 for r in bad]
+    s["value"][last, 0, 9] = float("nan")
+    moved = s["ring_k"].clone(), s["ring_v"].clone()
+    out = attention_call(s, dev, maps_of(dev, n), W, 0.0625, moved)
+    nodes = [r * n + i for r in some for i in range(n)]
+    within(clean[nodes], want[nodes], slack[nodes], 2.0 ** -8, "without it")
+    rest = [i for i in nodes if i not in last]
+    within(out[rest], want[rest], slack[rest], 2.0 ** -8, "the other nodes")
+    others = [r * n + i for r in range(rows_n) if r not in bad for i in range(n)]
+    assert torch.equal(out[others], clean[others])
+    dims = out[last].reshape(len(bad), G, D)
+    assert not torch.isfinite(dims[:, :, 9]).any()
+    keep = [g * D + d for g in range(G) for d in range(D) if d != 9]
+    within(out[last][:, keep], want[last][:, keep], slack[last][:, keep], 2.0 ** -8, "its other dims")
+    ref = s["ring_k"].clone(), s["ring_v"].clone()
+    for r in range(rows_n):
+        for j in range(commits[r]):
+            for x, y in zip(ref, (s["new_k"], s["value"])):
+                x[slots[r], :, (starts[r] + j) % W] = y[r * n + j]
+    for x, y in zip(moved, ref):
+        assert torch.equal(x, y)
+    for x, y in zip(rings, ref):
+        assert torch.equal(x, y)
+
+
+def test_attention_takes_tokens_that_lie_apart():
+    """q, new_k, value and the gate as columns of one wider projection: bitwise the packed ones."""
+    lens, hkv, G, W = [7, 30], 2, 3, 512
+    _, slots, starts, pool_rows, dev = batch(12, lens, True)
+    total, hq = sum(lens), hkv * G
+    s = attention_inputs(12, total, pool_rows, slots, starts, hkv, G, W)
+    before = s["ring_k"].clone(), s["ring_v"].clone()
+    rings = tuple(x.clone() for x in before)
+    want = attention_call(s, dev, maps_of(dev), W, 0.0625, rings)
+    widths = {"q": hq * D, "new_k": hkv * D, "value": hkv * D, "gate": hq * 2 * D}
+    wide = randn(3, total, sum(widths.values()) + 24)
+    at, t = 8, dict(s)
+    for name, w in widths.items():
+        wide[:, at:at + w] = s[name].reshape(total, w)
+        t[name] = wide[:, at:at + w].unflatten(1, s[name].shape[1:]) if s[name].dim() > 2 else wide[:, at:at + w]
+        at += w
+    assert not t["q"].is_contiguous()
+    other = tuple(x.clone() for x in before)
+    assert torch.equal(attention_call(t, dev, maps_of(dev), W, 0.0625, other), want)
+    for x, y in zip(rings, other):
+        assert torch.equal(x, y)
 
 
 def test_attention_leaves_the_rest_alone():
@@ -532,6 +622,42 @@ def test_run_on_another_stream_and_shared_slots():
         alone = layers(one, d1, H, HV, W, 16)
         for a, b in zip(alone[1:], want[1:]):
             assert torch.equal(a, b[at])
+
+
+def test_two_streams_at_once_and_a_workspace_of_two_graphs():
+    """Lone rows, whose attention splits its keys over a workspace: calls of two streams that overlap, and two graphs over one
+    workspace replayed in turn, give what each gives alone."""
+    hkv, G, W = 2, 4, 512
+    sides = []
+    for k in (1, 2):
+        rows, slots, starts, pool_rows, dev = batch(60 + k, [11 + k], False)
+        s = attention_inputs(70 + k, 11 + k, pool_rows, slots, starts, hkv, G, W)
+        trees = maps_of(dev, 16)
+        sides.append((s, dev, trees, attention_call(s, dev, trees, W, 0.0625)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sides]
+    got = [[], []]
+    for _ in range(12):
+        for k, (s, dev, trees, _) in enumerate(sides):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(attention_call(s, dev, trees, W, 0.0625))
+    torch.cuda.synchronize()
+    for k, (_, _, _, want) in enumerate(sides):
+        assert all(torch.equal(x, want) for x in got[k])
+    from hs_guard._lib import lib
+    space = torch.empty(lib().hsg_tree_attention_workspace_bytes(1, hkv, G, 16), dtype=torch.uint8, device="cuda")
+    assert space.numel() > 0
+    graphs = []
+    for s, dev, trees, _ in sides:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = attention_call(s, dev, trees, W, 0.0625, workspace=space)
+        graphs.append((graph, out))
+    for _ in range(3):
+        for (graph, out), (_, _, _, want) in zip(graphs, sides):
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, want)
 
 
 def test_refusals():
