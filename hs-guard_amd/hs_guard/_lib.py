@@ -201,6 +201,7 @@ def lib():
 
 
 _calls = None
+_tensor_checks = None
 
 
 def calls():
@@ -216,6 +217,20 @@ def calls():
                                "(run `python -c 'import __graft_entry__ as g; g.build()'` at the repo root)") from e
         _calls = _hsgcall
     return _calls
+
+
+def tensor_checks():
+    """The native checks of the operators' tensors (hs_guard._hsgtensor): ``operands`` and ``row_stride``."""
+    global _tensor_checks
+    if _tensor_checks is None:
+        import torch  # noqa: F401  (its libraries, which the module is linked to)
+        try:
+            from . import _hsgtensor
+        except ImportError as e:
+            raise RuntimeError(f"HS-Guard native tensor checks not built: {e} "
+                               "(run `python -c 'import __graft_entry__ as g; g.build()'` at the repo root)") from e
+        _tensor_checks = _hsgtensor
+    return _tensor_checks
 
 
 def check(rc, name):

@@ -11,7 +11,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from .._lib import HSG_GDN_BURST_MIN_DEFAULT, HSG_TREE_MAX_NODES, calls, check, lib
+from .._lib import HSG_GDN_BURST_MIN_DEFAULT, HSG_TREE_MAX_NODES, calls, check, lib, tensor_checks
 
 HSG_STATE_F32 = 0
 HSG_STATE_F16 = 1
@@ -338,58 +338,12 @@ class DraftTrees(NamedTuple):
     max_nodes: int = HSG_TREE_MAX_NODES     # bound on every row's nodes; smaller bounds take smaller tiles
 
 
-_I64 = torch.int64
 _current_device = torch._C._cuda_getDevice
 
 
-def _device_of(*tensors):
-    """The index of the one GPU that the tensors (None skipped) are on."""
-    index = tensors[0].get_device()
-    if index < 0:
-        raise AssertionError("HS-Guard kernels take GPU tensors")
-    for t in tensors:
-        if t is not None and t.get_device() != index:
-            raise AssertionError("tensors must be on one GPU")
-    return index
-
-
-def _index_tensors(*tensors):
-    """The index tensors (None skipped) are contiguous int64."""
-    for t in tensors:
-        if t is not None and (t.dtype is not _I64 or not t.is_contiguous()):
-            raise AssertionError("index tensors must be contiguous int64")
-
-
-def _tree_rows(trees, slots, tokens):
-    """Checks a batch of trees over ``tokens`` packed tokens; returns its rows."""
-    offsets, lens, commits, _, masks, most = trees
-    _index_tensors(slots, offsets, lens, commits, masks)
-    shape = slots.shape
-    if len(shape) != 1 or offsets.shape != shape or lens.shape != shape or (commits is not None
-                                                                           and commits.shape != shape):
-        raise AssertionError("offsets, lens, commits and slots must be [n]")
-    if masks.shape != (tokens,):
-        raise AssertionError("masks must be [T], one for each packed token")
+def _node_bound(most):
     if not 1 <= most <= HSG_TREE_MAX_NODES:
         raise AssertionError(f"max_nodes must be in [1, {HSG_TREE_MAX_NODES}]")
-    return shape[0]
-
-
-def _packed_rows(t, tokens, width):
-    """t [tokens, ...] bf16 holds each token's ``width`` values next to one another: how far apart its tokens lie."""
-    if t.dtype is not torch.bfloat16 or t.shape[0] != tokens or t.numel() != tokens * width:
-        raise AssertionError(f"[{tokens}, {width}] bf16 values expected, got {list(t.shape)} of {t.dtype}")
-    if t.is_contiguous():
-        return width
-    inner = 1
-    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-        if size != 1 and stride != inner:
-            raise AssertionError("a token's values must be contiguous")
-        inner *= size
-    stride = t.stride(0) if tokens > 1 else width
-    if stride < width:
-        raise AssertionError("tokens must not overlap")
-    return stride
 
 
 def _launch(name, device, *args):
@@ -411,22 +365,17 @@ def draft_tree_maps(parents, lens, starts, commits=None, max_nodes=HSG_TREE_MAX_
     int64: nodes of each row, tokens its session holds, leading nodes to commit. A row that is no tree (a parent that does
     not come before its child, more than ``max_nodes`` nodes or more than the buffer holds, commits that are no chain from
     the session's last token) comes back with lens and commits 0. pos and masks of tokens of no row are 0."""
-    device = _device_of(parents, lens, starts, commits)
-    _index_tensors(parents, lens, starts, commits)
-    shape = lens.shape
-    if parents.dim() != 1 or len(shape) != 1 or starts.shape != shape or (commits is not None and commits.shape != shape):
-        raise AssertionError("parents must be [T]; lens, starts and commits [n]")
-    if not 1 <= max_nodes <= HSG_TREE_MAX_NODES:
-        raise AssertionError(f"max_nodes must be in [1, {HSG_TREE_MAX_NODES}]")
-    n, total = shape[0], parents.shape[0]
+    n, total = lens.numel(), parents.numel()
+    device, p_parents, p_lens, p_starts, p_commits = tensor_checks().operands("tnnn", n, total, parents, lens, starts, commits)
+    _node_bound(max_nodes)
     # (one allocation for all: a small batch's cost is this function's own)
     if commits is None:
         commits_out = None
         offsets, lens_out, pos, masks = parents.new_empty(2 * (n + total)).split((n, n, total, total))
     else:
         offsets, lens_out, commits_out, pos, masks = parents.new_empty(3 * n + 2 * total).split((n, n, n, total, total))
-    _launch("hsg_tree_maps", device, parents.data_ptr(), total, lens.data_ptr(), starts.data_ptr(), _ptr(commits), n,
-            max_nodes, offsets.data_ptr(), lens_out.data_ptr(), _ptr(commits_out), pos.data_ptr(), masks.data_ptr())
+    _launch("hsg_tree_maps", device, p_parents, total, p_lens, p_starts, p_commits, n, max_nodes, offsets.data_ptr(),
+            lens_out.data_ptr(), _ptr(commits_out), pos.data_ptr(), masks.data_ptr())
     return DraftTrees(offsets, lens_out, commits_out, pos, masks, max_nodes)
 
 
@@ -435,19 +384,21 @@ def tree_conv_silu(qkv, pool, weight, slots, trees):
     (rows may lie further apart), pool [S, 3, C] bf16 (one layer), weight [C, 1, 4] bf16. Returns [T, C] bf16; tokens of no
     row are not written. Rows that commit move their history in ``pool`` and need slots of their own."""
     total, c = qkv.shape
-    device = _device_of(qkv, pool, weight, slots, *trees[:5])
-    stride = _packed_rows(qkv, total, c)
-    _bf16_in(pool, weight)
+    n = slots.numel()
+    offsets, lens, commits, _, masks, most = trees
+    checks = tensor_checks()
+    device, p_x, p_pool, p_weight, p_slots, p_offsets, p_lens, p_commits, p_masks = checks.operands(
+        "pbbnnnnt", n, total, qkv, pool, weight, slots, offsets, lens, commits, masks)
+    _node_bound(most)
+    stride = checks.row_stride(qkv, total, c)
     ks = weight.shape[-1]
     if pool.dim() != 3 or pool.shape[1] != ks - 1 or pool.shape[2] != c or weight.numel() != c * ks:
         raise AssertionError("tree_conv_silu: pool [S, K-1, C], weight [C, 1, K]")
-    n = _tree_rows(trees, slots, total)
     out = qkv.new_empty((total, c))
     if not total:
         return out
-    _launch("hsg_tree_conv_silu", device, qkv.data_ptr(), stride, pool.data_ptr(), pool.shape[0], weight.data_ptr(), ks,
-            slots.data_ptr(), trees.lens.data_ptr(), trees.offsets.data_ptr(), _ptr(trees.commits), trees.masks.data_ptr(),
-            n, trees.max_nodes, c, out.data_ptr(), c)
+    _launch("hsg_tree_conv_silu", device, p_x, stride, p_pool, pool.shape[0], p_weight, ks, p_slots, p_lens, p_offsets,
+            p_commits, p_masks, n, most, c, out.data_ptr(), c)
     return out
 
 
@@ -460,32 +411,33 @@ def gdn_tree_step(packed, key_dim, heads, head_k, value_heads, head_v, a, b, A_l
     that commit move their state and need slots of their own; no other state is written."""
     total = packed.shape[0]
     hvv = value_heads * head_v
-    device = _device_of(packed, a, b, A_log, dt_bias, state, slots, z, norm_weight, *trees[:5])
-    stride = _packed_rows(packed, total, 2 * key_dim + hvv)
-    ab = _packed_rows(a, total, value_heads)
-    if key_dim != heads * head_k or _packed_rows(b, total, value_heads) != ab:
+    n = slots.numel()
+    offsets, lens, commits, _, masks, most = trees
+    checks = tensor_checks()
+    device, p_packed, p_a, p_b, p_log, p_bias, p_state, p_z, p_norm, p_slots, p_offsets, p_lens, p_commits, p_masks = \
+        checks.operands("pppbbspbnnnnt", n, total, packed, a, b, A_log, dt_bias, state, z, norm_weight, slots, offsets, lens,
+                        commits, masks)
+    _node_bound(most)
+    stride, ab = checks.row_stride(packed, total, 2 * key_dim + hvv), checks.row_stride(a, total, value_heads)
+    if key_dim != heads * head_k or checks.row_stride(b, total, value_heads) != ab:
         raise AssertionError("key_dim must be heads * head_k, and a and b have one row stride")
-    _bf16_in(A_log, dt_bias)
     if A_log.numel() != value_heads or dt_bias.numel() != value_heads:
         raise AssertionError("A_log and dt_bias must be [HV]")
-    if state.dtype not in _STATE_CODES or not state.is_contiguous() or state.shape[1:] != (value_heads, head_k, head_v):
-        raise AssertionError("state must be contiguous [S, HV, K, V], float32 or float16")
+    if state.shape[1:] != (value_heads, head_k, head_v):
+        raise AssertionError("state must be [S, HV, K, V]")
     if (z is None) != (norm_weight is None):
         raise AssertionError("the gated norm takes z and norm_weight")
     z_stride = 0
     if z is not None:
-        z_stride = _packed_rows(z, total, hvv)
-        _bf16_in(norm_weight)
+        z_stride = checks.row_stride(z, total, hvv)
         _require(norm_weight.numel() == head_v, "norm_weight must be [V]")
-    n = _tree_rows(trees, slots, total)
     out = packed.new_empty((total, hvv))
     if not total:
         return out
-    _launch("hsg_gdn_tree_step", device, packed.data_ptr(), stride, 0, key_dim, 2 * key_dim, a.data_ptr(), b.data_ptr(), ab,
-            A_log.data_ptr(), dt_bias.data_ptr(), state.data_ptr(), _STATE_CODES[state.dtype], state.shape[0],
-            slots.data_ptr(), trees.lens.data_ptr(), trees.offsets.data_ptr(), _ptr(trees.commits), trees.masks.data_ptr(),
-            n, trees.max_nodes, heads, value_heads, head_k, head_v, head_k ** -0.5 if scale is None else float(scale),
-            _ptr(z), z_stride, _ptr(norm_weight), float(eps), out.data_ptr())
+    _launch("hsg_gdn_tree_step", device, p_packed, stride, 0, key_dim, 2 * key_dim, p_a, p_b, ab, p_log, p_bias, p_state,
+            _STATE_CODES[state.dtype], state.shape[0], p_slots, p_lens, p_offsets, p_commits, p_masks, n, most, heads,
+            value_heads, head_k, head_v, head_k ** -0.5 if scale is None else float(scale), p_z, z_stride, p_norm, float(eps),
+            out.data_ptr())
     return out
 
 
@@ -499,33 +451,34 @@ def tree_ring_attention(q, ring_k, ring_v, new_k, value, gate, ring_pos, slots, 
     tensor of hsg_tree_attention_workspace_bytes, which calls of few rows use (allocated per call when None)."""
     total, hq, d = q.shape
     hkv = new_k.shape[1]
-    device = _device_of(q, ring_k, ring_v, new_k, value, gate, ring_pos, slots, starts, workspace, *trees[:5])
+    n = slots.numel()
+    offsets, lens, commits, _, masks, most = trees
+    checks = tensor_checks()
+    device, p_q, p_rk, p_rv, p_k, p_v, p_gate, p_pos, p_starts, p_slots, p_offsets, p_lens, p_commits, p_masks, space = \
+        checks.operands("pbbpppinnnnntu", n, total, q, ring_k, ring_v, new_k, value, gate, ring_pos, starts, slots, offsets,
+                        lens, commits, masks, workspace)
+    _node_bound(most)
     if hkv == 0 or hq % hkv:
         raise AssertionError("query heads must be a multiple of the kv heads")
     groups = hq // hkv
-    qs, ks, vs = _packed_rows(q, total, hq * d), _packed_rows(new_k, total, hkv * d), _packed_rows(value, total, hkv * d)
-    gs = 0 if gate is None else _packed_rows(gate, total, hq * 2 * d)
-    _bf16_in(ring_k, ring_v)
+    qs, ks, vs = (checks.row_stride(q, total, hq * d), checks.row_stride(new_k, total, hkv * d),
+                  checks.row_stride(value, total, hkv * d))
+    gs = 0 if gate is None else checks.row_stride(gate, total, hq * 2 * d)
     rings = ring_k.shape
     if len(rings) != 4 or rings[1:] != (hkv, window + 1, d) or ring_v.shape != rings:
         raise AssertionError("ring_k and ring_v must be [S, Hkv, W+1, D]")
     if ring_pos.shape != (rings[0], window + 1):
         raise AssertionError("ring_pos must be [S, W+1]")
-    _index_tensors(ring_pos, starts)
-    n = _tree_rows(trees, slots, total)
-    _require(starts.shape == slots.shape, "starts must be [n]")
     out = q.new_empty((total, hq * d))
     if not total:
         return out
-    most = trees.max_nodes
     if workspace is None:
         need = lib().hsg_tree_attention_workspace_bytes(n, hkv, groups, most)
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    else:
-        _require(workspace.dtype is torch.uint8 and workspace.is_contiguous(), "workspace must be contiguous uint8")
-    _launch("hsg_tree_attention", device, q.data_ptr(), qs, groups * d, d, ring_k.data_ptr(), ring_v.data_ptr(), rings[0],
-            window, new_k.data_ptr(), ks, d, value.data_ptr(), vs, d, _ptr(gate), gs, groups * 2 * d, 2 * d, d,
-            ring_pos.data_ptr(), slots.data_ptr(), starts.data_ptr(), trees.lens.data_ptr(), trees.offsets.data_ptr(),
-            _ptr(trees.commits), trees.masks.data_ptr(), n, most, hkv, groups, d, float(scale), out.data_ptr(), hq * d,
-            groups * d, d, _ptr(workspace), 0 if workspace is None else workspace.numel())
+        if need:
+            workspace = q.new_empty(need, dtype=torch.uint8)
+            space = workspace.data_ptr()
+    _launch("hsg_tree_attention", device, p_q, qs, groups * d, d, p_rk, p_rv, rings[0], window, p_k, ks, d, p_v, vs, d, p_gate,
+            gs, groups * 2 * d, 2 * d, d, p_pos, p_slots, p_starts, p_lens, p_offsets, p_commits, p_masks, n, most, hkv,
+            groups, d, float(scale), out.data_ptr(), hq * d, groups * d, d, space,
+            0 if workspace is None else workspace.numel())
     return out

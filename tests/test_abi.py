@@ -227,3 +227,28 @@ def test_tree_operators_refuse_before_launch():
     assert need(1, 4, 4, 12) == 4 * 8 * 48 * 258 * 4      # 4 kv heads, 8 splits, 48 query rows of 256 sums, maximum, weight
     assert need(12, 4, 4, 12) == 12 * 4 * 4 * 48 * 258 * 4 and need(20, 4, 4, 12) == 0
     assert need(352, 4, 4, 12) == 0 and need(0, 4, 4, 12) == 0 and need(1, 4, 4, 65) == 0
+
+
+def test_tensor_checks_on_the_host():
+    """Strides of packed tokens, and refusals that need no GPU: tensors on the host, things that are no tensors, kinds that do
+    not fit the arguments."""
+    import torch
+
+    from hs_guard._lib import tensor_checks
+    C = tensor_checks()
+    wide = torch.zeros(5, 40, dtype=torch.bfloat16)
+    for t, tokens, width, want in ((wide, 5, 40, 40), (wide[:, :24], 5, 24, 40), (wide[:, 8:32].unflatten(1, (3, 8)), 5, 24, 40),
+                                   (wide[:1, :24], 1, 24, 24), (wide[::2, :8], 3, 8, 80), (wide[:0], 0, 40, 40),
+                                   (wide.view(5, 1, 40), 5, 40, 40)):
+        assert C.row_stride(t, tokens, width) == want
+    for t, tokens, width in ((wide, 5, 39), (wide, 4, 50), (wide.t(), 40, 5), (wide[:, ::2], 5, 20),
+                             (wide.view(5, 4, 10)[:, :2, :5], 5, 10), (wide[:1, :24].expand(5, 24), 5, 24),
+                             (torch.zeros(()), 1, 1)):
+        with pytest.raises(AssertionError):
+            C.row_stride(t, tokens, width)
+    with pytest.raises((AssertionError, TypeError)):
+        C.row_stride(3, 1, 1)
+    assert C.operands("pi", 1, 1, None, None) == (-1, None, None)
+    for args in (("p", 1, 1, wide), ("p", 1, 1, 7), ("pp", 1, 1, None), ("p", 1, 1), ("p", "1", 1, None), (1, 1, 1, None)):
+        with pytest.raises((AssertionError, TypeError)):
+            C.operands(*args)
