@@ -202,14 +202,13 @@ extern "C" int hsg_tree_maps(const int64_t* parents, int64_t tokens, const int64
                              int64_t* lens_out, int64_t* commits_out, int64_t* pos, int64_t* masks, void* stream) {
   using namespace hsg;
   if (n_rows < 0 || tokens < 0 || tokens > ((int64_t)1 << 40)) return HSG_ERR_ARG;
-  if (max_nodes <= 0 || max_nodes > MOST) return HSG_ERR_SHAPE;
+  if (max_nodes <= 0 || max_nodes > MOST || n_rows > 65535) return HSG_ERR_SHAPE;   // (the sums before a row grow as rows^2)
   if (n_rows == 0 && tokens == 0) return HSG_OK;
   if (n_rows && (!lens || !starts || !offsets || !lens_out || (commits && !commits_out))) return HSG_ERR_ARG;
   if (tokens && (!parents || !pos || !masks)) return HSG_ERR_ARG;
   // every workgroup reads lens while others write
   if (n_rows && (lens_out == lens || offsets == lens || (commits && commits_out == lens))) return HSG_ERR_ARG;
   const unsigned blocks = n_rows ? ((unsigned)n_rows + ROWS_PER_WG - 1) / ROWS_PER_WG : 1;
-  if (blocks >= (1u << 24)) return HSG_ERR_SHAPE;   // a launch holds less than 2^32 threads
   hipLaunchKernelGGL(tree_maps_kernel, dim3(blocks), dim3(64 * ROWS_PER_WG), 0, reinterpret_cast<hipStream_t>(stream),
                      parents, tokens, lens, starts, commits, n_rows, max_nodes, offsets, lens_out,
                      commits ? commits_out : nullptr, pos, masks);

@@ -534,7 +534,8 @@ int hsg_gemm_blas_version(void);
  *   negative start, commits outside [0, lens[n]] or over nodes that are no chain);  pos[t] = starts[n] + depth (the roots'
  *   is 0);  masks[t] as above; pos and masks of tokens of no row are 0.
  *   parents, pos, masks [tokens] int64; lens, starts, commits, offsets, lens_out, commits_out [n_rows] int64 (commits and
- *   commits_out may be NULL). The outputs must not overlap the inputs. One launch. Supported: max_nodes <= 64.
+ *   commits_out may be NULL). The outputs must not overlap the inputs. One launch. Supported: max_nodes <= 64, at
+ *   most 65,535 rows.
  */
 int hsg_tree_maps(const int64_t* parents, int64_t tokens, const int64_t* lens, const int64_t* starts,
                   const int64_t* commits, int32_t n_rows, int32_t max_nodes, int64_t* offsets, int64_t* lens_out,

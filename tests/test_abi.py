@@ -177,7 +177,7 @@ def test_tree_operators_refuse_before_launch():
                                masks, None)
 
     assert maps(rows=0, tokens=0) == 0
-    assert [maps(most=m) for m in (0, 65)] == [SHAPE, SHAPE]
+    assert [maps(most=m) for m in (0, 65)] == [SHAPE, SHAPE] and maps(rows=65536) == SHAPE
     for bad in ({"rows": -1}, {"tokens": -1}, {"parents": None}, {"lens": None}, {"starts": None}, {"commits_out": None},
                 {"lens_out": 256}, {"offsets": 256}, {"pos": None}, {"masks": None}):
         assert maps(**bad) == ARG, bad

@@ -136,6 +136,29 @@ def test_conv(lens, channels, commit, gap):
         np.testing.assert_array_equal(_f64(got_pool), pool2)
 
 
+@pytest.mark.parametrize("most", [1, 7, 16, 29, 32, 64])
+@pytest.mark.parametrize("rows_n,channels", [(33, 520), (90, 1032)])
+def test_conv_over_many_rows(most, rows_n, channels):
+    """The tiles that calls of many rows take, by the bound on a row's nodes; in place, bitwise the same."""
+    from hs_guard._lib import calls
+    from hs_guard.engine.kernels import tree_conv_silu
+    lens = np.random.default_rng(most + rows_n).integers(0, most + 1, rows_n).tolist()
+    lens[5] = most
+    rows, slots, _, pool_rows, dev = batch(rows_n + most, lens, True, 2)
+    x, w = randn(1, dev["parents"].numel(), channels), randn(3, channels, 1, 4, scale=0.5)
+    pool = randn(2, pool_rows, 3, channels)
+    want, size, pool2 = tree.tree_conv_silu(_f64(x), _f64(pool), _f64(w), slots, rows)
+    t, live, got_pool, same_pool = maps_of(dev, most), sum(lens), pool.clone(), pool.clone()
+    out = tree_conv_silu(x, got_pool, w, dev["slots"], t)
+    within(out[:live], want[:live], 2.0 ** -20 * size[:live], 2.0 ** -8, "out")
+    np.testing.assert_array_equal(_f64(got_pool), pool2)
+    assert calls().hsg_tree_conv_silu(x.data_ptr(), channels, same_pool.data_ptr(), pool_rows, w.data_ptr(), 4,
+                                      dev["slots"].data_ptr(), t.lens.data_ptr(), t.offsets.data_ptr(),
+                                      t.commits.data_ptr(), t.masks.data_ptr(), rows_n, most, channels, x.data_ptr(),
+                                      channels, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(x[:live], out[:live]) and torch.equal(same_pool, got_pool)
+
+
 def test_conv_leaves_the_rest_alone_and_runs_in_place():
     """Rows of an unknown slot and tokens of no row keep their outputs; out may be the input."""
     from hs_guard._lib import calls
