@@ -366,14 +366,14 @@ def draft_tree_maps(parents, lens, starts, commits=None, max_nodes=HSG_TREE_MAX_
     not come before its child, more than ``max_nodes`` nodes or more than the buffer holds, commits that are no chain from
     the session's last token) comes back with lens and commits 0. pos and masks of tokens of no row are 0."""
     n, total = lens.numel(), parents.numel()
-    device, p_parents, p_lens, p_starts, p_commits = tensor_checks().operands("tnnn", n, total, parents, lens, starts, commits)
+    checks = tensor_checks()
+    device, p_parents, p_lens, p_starts, p_commits = checks.operands("tnnn", n, total, parents, lens, starts, commits)
     _node_bound(max_nodes)
-    # (one allocation for all: a small batch's cost is this function's own)
+    commits_out = None
     if commits is None:
-        commits_out = None
-        offsets, lens_out, pos, masks = parents.new_empty(2 * (n + total)).split((n, n, total, total))
+        offsets, lens_out, pos, masks = checks.empties(parents, n, n, total, total)
     else:
-        offsets, lens_out, commits_out, pos, masks = parents.new_empty(3 * n + 2 * total).split((n, n, n, total, total))
+        offsets, lens_out, commits_out, pos, masks = checks.empties(parents, n, n, n, total, total)
     _launch("hsg_tree_maps", device, p_parents, total, p_lens, p_starts, p_commits, n, max_nodes, offsets.data_ptr(),
             lens_out.data_ptr(), _ptr(commits_out), pos.data_ptr(), masks.data_ptr())
     return DraftTrees(offsets, lens_out, commits_out, pos, masks, max_nodes)
@@ -394,7 +394,7 @@ def tree_conv_silu(qkv, pool, weight, slots, trees):
     ks = weight.shape[-1]
     if pool.dim() != 3 or pool.shape[1] != ks - 1 or pool.shape[2] != c or weight.numel() != c * ks:
         raise AssertionError("tree_conv_silu: pool [S, K-1, C], weight [C, 1, K]")
-    out = qkv.new_empty((total, c))
+    out = checks.empty_rows(qkv, total, c)
     if not total:
         return out
     _launch("hsg_tree_conv_silu", device, p_x, stride, p_pool, pool.shape[0], p_weight, ks, p_slots, p_lens, p_offsets,
@@ -431,7 +431,7 @@ def gdn_tree_step(packed, key_dim, heads, head_k, value_heads, head_v, a, b, A_l
     if z is not None:
         z_stride = checks.row_stride(z, total, hvv)
         _require(norm_weight.numel() == head_v, "norm_weight must be [V]")
-    out = packed.new_empty((total, hvv))
+    out = checks.empty_rows(packed, total, hvv)
     if not total:
         return out
     _launch("hsg_gdn_tree_step", device, p_packed, stride, 0, key_dim, 2 * key_dim, p_a, p_b, ab, p_log, p_bias, p_state,
@@ -469,7 +469,7 @@ def tree_ring_attention(q, ring_k, ring_v, new_k, value, gate, ring_pos, slots, 
         raise AssertionError("ring_k and ring_v must be [S, Hkv, W+1, D]")
     if ring_pos.shape != (rings[0], window + 1):
         raise AssertionError("ring_pos must be [S, W+1]")
-    out = q.new_empty((total, hq * d))
+    out = checks.empty_rows(q, total, hq * d)
     if not total:
         return out
     if workspace is None:

@@ -252,3 +252,15 @@ def test_tensor_checks_on_the_host():
     for args in (("p", 1, 1, wide), ("p", 1, 1, 7), ("pp", 1, 1, None), ("p", 1, 1), ("p", "1", 1, None), (1, 1, 1, None)):
         with pytest.raises((AssertionError, TypeError)):
             C.operands(*args)
+    a, b, c = C.empties(torch.zeros(2, dtype=torch.long), 3, 0, 4)
+    a.fill_(1)
+    c.fill_(2)
+    assert (a.tolist(), b.tolist(), c.tolist()) == ([1] * 3, [], [2] * 4) and c.is_contiguous() and c.dtype is torch.long
+    out = C.empty_rows(wide[:, ::2], 3, 8)
+    assert out.shape == (3, 8) and out.is_contiguous() and out.dtype is torch.bfloat16
+    for bad in ((), (wide,), (3, 3), (wide, -1)):
+        with pytest.raises((AssertionError, TypeError)):
+            C.empties(*bad)
+    for bad in ((wide, 3), (wide, "3", 8), (wide, -1, 8)):
+        with pytest.raises((AssertionError, TypeError, RuntimeError)):
+            C.empty_rows(*bad)
