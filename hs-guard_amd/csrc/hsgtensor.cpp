@@ -1,7 +1,7 @@
-// What the operators' wrappers ask of their tensors, and their outputs, as Python functions (CPython extension hs_guard._hsgtensor, host code
-// only): device, type, layout and length of every operand and its address in one call. Asked one by one from Python this is
-// most of a small call: 13 operands 5.5 us, 0.3 here; a gated-delta step of one row 10.7 -> 6.6 us of host time, the attention
-// 15.4 -> 10.9, the maps (five outputs) 8.7 -> 6.1.
+// What the operators' wrappers ask of their tensors, and their outputs, as Python functions (CPython extension
+// hs_guard._hsgtensor, host code only): device, type, layout and length of every operand and its address in one call. Asked one
+// by one from Python this is most of a small call: 13 operands 5.5 us, 0.3 here; a gated-delta step of one row 10.7 -> 6.6 us
+// of host time, the attention 15.4 -> 10.9, the maps (five outputs) 8.7 -> 6.1.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <ATen/Functions.h>
