@@ -284,7 +284,8 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) raw[s][i] = *reinterpret_cast<const StatePair*>(state + (32 * s + i) * KD + state_lane);
+    for (int i = 0; i < 8; ++i)
+      raw[s][i] = __builtin_nontemporal_load(reinterpret_cast<const StatePair*>(state + (32 * s + i) * KD + state_lane));
   const auto s0 = [&](int s, int j, int i) {
     if constexpr (HALF) return h2f((uint16_t)(raw[s][i] >> (16 * j)));
     else return raw[s][i][j];
@@ -623,8 +624,8 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           StateValue* const at = state + (32 * s + 4 * hh + r) * KD + state_lane;
-          if constexpr (HALF) *reinterpret_cast<uint32_t*>(at) = (uint32_t)f2h(acc[0][r]) | ((uint32_t)f2h(acc[1][r]) << 16);
-          else *reinterpret_cast<f32x2*>(at) = (f32x2){acc[0][r], acc[1][r]};
+          if constexpr (HALF) __builtin_nontemporal_store((uint32_t)f2h(acc[0][r]) | ((uint32_t)f2h(acc[1][r]) << 16), reinterpret_cast<uint32_t*>(at));
+          else __builtin_nontemporal_store((f32x2){acc[0][r], acc[1][r]}, reinterpret_cast<f32x2*>(at));
         }
       }
     };

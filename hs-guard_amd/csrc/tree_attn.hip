@@ -103,7 +103,7 @@ __device__ __forceinline__ bf16x8 as_bf16x8(u32x4 w) { return __builtin_bit_cast
 __device__ __forceinline__ u32x4 load16(const uint16_t* p) { return *reinterpret_cast<const u32x4*>(p); }
 // 16 bytes at byte `off` of a base that is the same for all lanes: its address takes one register of a lane
 __device__ __forceinline__ u32x4 load16_at(const uint16_t* base, uint32_t off) {
-  return *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + off);
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + off));
 }
 // the largest of three, a NaN aside, in one instruction (fmaxf quiets its operands first, an instruction each)
 __device__ __forceinline__ float max3(float a, float b, float c) {
