@@ -15,7 +15,8 @@
 // Up to 16 query rows a (row, kv head), bound by reading the ring: the four waves split its KEYS, a wave's keys and values going
 // straight from memory to its operand registers (of a value 8 dims of a lane's 8 keys, whose 16-bit halves it swaps), and meet
 // in LDS at the end, weighted by their maxima; no barrier and no LDS write in the loop. 352 rows of one node over full rings, 16
-// q / 4 kv heads: 120 us, 5.5 TB/s.
+// q / 4 kv heads: 118 us, 5.6 TB/s (nontemporal loads; with ordinary ones 122, while keys through LDS, which other workgroups
+// read too, take 117 us with nontemporal and 105 with ordinary loads at 128 x 64).
 // More query rows: every wave has one or two tiles of its own and needs every key, so blocks pass through LDS once for the four
 // waves (two stages of 32 KB, direct-to-LDS loads, one barrier a block; two workgroups on a CU). Keys are read as they lie,
 // values by transpose reads, both ahead of their products, and waves at their products go before waves at their softmax. 128
@@ -796,7 +797,7 @@ __global__ __launch_bounds__(256) void tree_ring_write_kernel(const TreeAttnPara
   write_chain(p, blockIdx.x / p.hkv, blockIdx.x % p.hkv, blockIdx.y, gridDim.y);
 }
 
-// Query rows of a workgroup. Up to 16 the waves split their keys (352 x 1 node 122 us, against 127 through LDS); beyond, keys
+// Query rows of a workgroup. Up to 16 the waves split their keys (352 x 1 node 119 us, against 127 through LDS); beyond, keys
 // pass through LDS for 4 waves of one tile, or of two where that fills the chip (256 CUs) and wastes little. 64 x 64 nodes, 16 q
 // / 4 kv heads: 55 us with 128 rows, 68 with 64; 20 x 64 36 and 30; 100 x 33 (129 to 192 rows are three workgroups of 64) 84 and
 // 67.
