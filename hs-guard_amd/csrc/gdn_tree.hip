@@ -19,12 +19,11 @@
 // so U never leaves the registers; A, P and the inverses of A's diagonal blocks go through LDS as fp32.
 // G is summed and its differences taken in fp64: a steep decay early on a path must not cost the digits of the later ones.
 //
-// Bound by reading the state where trees are small (352 x 1 node, 16 value heads, fp32: 61 us, 6.1 TB/s; 68 without nontemporal
-// loads), by the issue of a CU's two or three workgroups where they are large: 128 x 64 nodes with commits 102 us for 380 MB. A
-// workgroup then
-// lives 22 us, 6.4 of them until its loads are there, 2.7 in the coefficients, 2.7 in the state's products, 1.8 in U, 2 in the
-// commit; its products alone are 4.7. LDS reads ahead of the products and priorities of the waves changed nothing; 8 waves of
-// 16 columns spilled (125 -> 166 us).
+// Bound by reading the state where trees are small (352 x 1 node, 16 value heads, fp32: 61 us, 6.1 TB/s; 68 without
+// nontemporal loads), by the issue of a CU's two or three workgroups where they are large: 128 x 64 nodes with commits 102 us
+// for 380 MB. A workgroup then lives 22 us, 6.4 of them until its loads are there, 2.7 in the coefficients, 2.7 in the
+// state's products, 1.8 in U, 2 in the commit; its products alone are 4.7. LDS reads ahead of the products and priorities of
+// the waves changed nothing; 8 waves of 16 columns spilled (125 -> 166 us).
 //
 // A masked pair has a coefficient of 0, which would carry a NaN or an infinity of one branch to all others: where a result
 // is not finite, the workgroup computes its row again by walking each node's own ancestors (walk_row).
@@ -222,8 +221,8 @@ constexpr int occupancy(int nt, bool half) {
 }
 
 // NT: tiles of 16 nodes. One tile over an fp32 state does not move it: S0's registers are free as it is split, and four
-// workgroups on a CU instead of three (352 x 1 node 61 against 70 us; with commits two tiles were as fast, 112 and 112 us, and at
-// 12 nodes faster, 154 and 157).
+// workgroups on a CU instead of three (352 x 1 node 61 against 70 us; with commits two tiles were as fast, 112 and 112 us,
+// and at 12 nodes faster, 154 and 157).
 template <int NT, bool HALF, bool GATED>
 __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(const TreeStepParams p) {
   constexpr bool MOVES = HALF || NT > 1;
@@ -625,7 +624,9 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           StateValue* const at = state + (32 * s + 4 * hh + r) * KD + state_lane;
-          if constexpr (HALF) __builtin_nontemporal_store((uint32_t)f2h(acc[0][r]) | ((uint32_t)f2h(acc[1][r]) << 16), reinterpret_cast<uint32_t*>(at));
+          if constexpr (HALF)
+            __builtin_nontemporal_store((uint32_t)f2h(acc[0][r]) | ((uint32_t)f2h(acc[1][r]) << 16),
+                                        reinterpret_cast<uint32_t*>(at));
           else __builtin_nontemporal_store((f32x2){acc[0][r], acc[1][r]}, reinterpret_cast<f32x2*>(at));
         }
       }

@@ -9,21 +9,22 @@
 //   S^T[key, query] = K . Q^T      a lane's column is one query: maxima, sums and rescales are per-lane scalars
 //   O^T[d, query] += V^T . P^T     B = P straight from the S^T accumulators (the product's key order is the lane's own)
 // The running maximum is moved only when a block's exceeds it by 2^8, so the accumulators are seldom rescaled; sums are fp32
-// and P is rounded to bf16 for its product (2^-9 of each weight, below the output's own rounding), the weights' sum taking it
-// as rounded.
+// and P is rounded to bf16 for its product (2^-8 of each weight at most, as the output's own rounding; over a row's keys they
+// average out), the weights' sum taking it as rounded.
 //
-// Up to 16 query rows a (row, kv head), bound by reading the ring: the four waves split its KEYS, a wave's keys and values going
-// straight from memory to its operand registers (of a value 8 dims of a lane's 8 keys, whose 16-bit halves it swaps), and meet
-// in LDS at the end, weighted by their maxima; no barrier and no LDS write in the loop. 352 rows of one node over full rings, 16
-// q / 4 kv heads: 118 us, 5.6 TB/s (nontemporal loads; with ordinary ones 122, while keys through LDS, which other workgroups
-// read too, take 117 us with nontemporal and 105 with ordinary loads at 128 x 64).
-// More query rows: every wave has one or two tiles of its own and needs every key, so blocks pass through LDS once for the four
-// waves (two stages of 32 KB, direct-to-LDS loads, one barrier a block; two workgroups on a CU). Keys are read as they lie,
-// values by transpose reads, both ahead of their products, and waves at their products go before waves at their softmax. 128
-// rows of 64 nodes with commits: 109 us, where the bytes alone take 78; a block of a workgroup takes 2.1 us, of which its 64 products a wave
-// are 0.9 for the two workgroups that share a SIMD, the rest softmax, LDS reads and the issue of the next block's loads; 5.5 us
-// before the loop (ring positions, queries, first block) and 6 after it (gates, outputs) are not hidden. Operands by byte
-// permutes instead of transpose reads and reads right before their products made it 131 us; four tiles a wave spilled: 1,040 us.
+// Up to 16 query rows a (row, kv head), bound by reading the ring: the four waves split its KEYS, a wave's keys and values
+// going straight from memory to its operand registers (of a value 8 dims of a lane's 8 keys, whose 16-bit halves it swaps),
+// and meet in LDS at the end, weighted by their maxima; no barrier and no LDS write in the loop. 352 rows of one node over
+// full rings, 16 q / 4 kv heads: 118 us, 5.6 TB/s (nontemporal loads; with ordinary ones 122, while keys through LDS, which
+// other workgroups read too, take 117 us with nontemporal and 105 with ordinary loads at 128 x 64).
+// More query rows: every wave has one or two tiles of its own and needs every key, so blocks pass through LDS once for the
+// four waves (two stages of 32 KB, direct-to-LDS loads, one barrier a block; two workgroups on a CU). Keys are read as they
+// lie, values by transpose reads, both ahead of their products, and waves at their products go before waves at their softmax.
+// 128 rows of 64 nodes with commits: 109 us, where the bytes alone take 78; a block of a workgroup takes 2.1 us, of which its
+// 64 products a wave are 0.9 for the two workgroups that share a SIMD, the rest softmax, LDS reads and the issue of the next
+// block's loads; 5.5 us before the loop (ring positions, queries, first block) and 6 after it (gates, outputs) are not
+// hidden. Operands by byte permutes instead of transpose reads and reads right before their products made it 131 us; four
+// tiles a wave spilled: 1,040 us.
 // Where few rows leave the chip short of workgroups, workgroups split a row's key blocks further and a second launch joins
 // their partial sums: a lone row of 12 nodes 9.4 + 3.7 us, both a chain of dependent loads.
 //
@@ -253,6 +254,10 @@ __device__ __forceinline__ void write_chain(const TreeAttnParams& p, int n, int 
 // byte offset of an LDS pointer
 __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+__device__ __forceinline__ const uint16_t* lds_pointer(uint32_t byte) {
+  return (const uint16_t*)(const __attribute__((address_space(3))) uint16_t*)(uintptr_t)byte;
 }
 
 // 1 KB from memory into LDS without a register between: lane l's 16 bytes at byte `off` of `base` go to byte `to` + 16 l.
@@ -605,7 +610,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(const TreeAttnPar
         const uint32_t v_lds = lds_offset(v_at);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const uint16_t* const at = (const uint16_t*)(const __attribute__((address_space(3))) uint16_t*)(uintptr_t)(v_lds ^ (8 * i));
+          const uint16_t* const at = lds_pointer(v_lds ^ (8 * i));
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh) {
             const u32x2 lo = ld_tr4(at + 128 * hh), hi = ld_tr4(at + 128 * hh + 16 * D);
