@@ -576,7 +576,8 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
   if (MOVES && ro.done > 0) {
     const float ec = lds.eG[ro.done - 1];
     constexpr int NP = (NT + 1) / 2;     // pairs of tiles: a product takes 32 nodes, the lane's own 4 of either tile
-    bf16x8 up[NP][2][3];
+    constexpr int U_PARTS = HALF ? 2 : 3;   // to an fp16 state, which keeps 11 digits, 16 of u (96 x 33 nodes 82 -> 80 us)
+    bf16x8 up[NP][2][U_PARTS];
 #pragma unroll
     for (int t2 = 0; t2 < NP; ++t2) {
       float x[2][8] = {};
@@ -592,7 +593,7 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
           for (int j = 0; j < 2; ++j) x[j][4 * hh + r] = i0 + r < ro.done ? u[t][j][r] * (le[r] * ki[r]) : 0.f;
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) split8<3>(x[j], up[t2][j]);
+      for (int j = 0; j < 2; ++j) split8<U_PARTS>(x[j], up[t2][j]);
     }
     // state rows 32 s ..: accumulator row 4 g4 + r is state row 32 s + 8 g4 + 4 hh + r, operand row m = c is k's dim 32 s +
     // 8 (c / 4) + 4 hh + c % 4, which transpose reads of 4-value vectors 8 dims apart give
@@ -616,7 +617,7 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
           if (2 * t2 + 1 < NT) hi = four(2 * t2 + 1 < NT ? 2 * t2 + 1 : 0);
           const bf16x8 kf = __builtin_bit_cast(bf16x8, (u32x4){lo[0], lo[1], hi[0], hi[1]});
 #pragma unroll
-          for (int w = 2; w >= 0; --w)
+          for (int w = U_PARTS - 1; w >= 0; --w)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
               acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, up[t2][j][w], acc[j], 0, 0, 0);
