@@ -251,14 +251,15 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
 
   // Loads are waited for in the order of their issue: what the first phases need is loaded before S0, what the last ones need
   // after it.
-  // ---- the tiles of k, then of q, dealt over the waves ----
-  constexpr int EACH = (2 * NT + NW - 1) / NW;
+  // ---- the tiles of k, then of q, dealt over the waves but the first, which has the nodes' scalars ----
+  constexpr int EACH = (2 * NT + NW - 2) / (NW - 1);
+  const int first_job = wave ? wave - 1 : 2 * NT;
   // (lane offsets are 32 bits on a uniform base: 64-bit addresses per lane cost the registers of a workgroup on the CU)
   const uint32_t stride = (uint32_t)p.qkv_stride;
   u32x4 kq[EACH][4];
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    const int job = wave + NW * e;
+    const int job = first_job + (NW - 1) * e;
     if (job >= 2 * NT) break;
     const uint16_t* const src = job >= NT ? ro.q : ro.k;
     const uint32_t row = (uint32_t)min(16 * (job % NT) + c, len - 1) * stride + 8 * g4;
@@ -315,7 +316,7 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
   // ---- k and q to LDS, and their lengths ----
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    const int job = wave + NW * e;
+    const int job = first_job + (NW - 1) * e;
     if (job >= 2 * NT) break;
     const bool is_q = job >= NT;
     const int row = 16 * (job % NT) + c;
