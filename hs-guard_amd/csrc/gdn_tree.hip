@@ -292,24 +292,34 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
     else return raw[s][i][j];
   };
   // ---- v and z ----
-  uint32_t vw[NT][4], zw[GATED ? NT : 1][4];
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = min(16 * t + 4 * g4 + r, len - 1);
-      vw[t][r] = *reinterpret_cast<const uint32_t*>(ro.v + ((uint32_t)i * stride + col));
-    }
-  uint32_t nw = 0;
-  if constexpr (GATED) {
-    nw = *reinterpret_cast<const uint32_t*>(p.norm_w + col);
+  // A wave has at most 63 loads on their way: with more than a tile it would stand here until the first are back, so that
+  // there v is loaded after the first barrier and z after the state's products (96 x 33 76 -> 73 us, 128 x 64 106 -> 103.5).
+  constexpr bool LATE = NT > 1;
+  uint32_t vw[NT][4], zw[GATED ? NT : 1][4], nw = 0;
+  const auto load_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = min(16 * t + 4 * g4 + r, len - 1);
-        zw[t][r] = *reinterpret_cast<const uint32_t*>(ro.z + ((uint32_t)i * (uint32_t)p.z_stride + col));
+        vw[t][r] = *reinterpret_cast<const uint32_t*>(ro.v + ((uint32_t)i * stride + col));
       }
+  };
+  const auto load_z = [&]() __attribute__((always_inline)) {
+    if constexpr (GATED) {
+      nw = *reinterpret_cast<const uint32_t*>(p.norm_w + col);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = min(16 * t + 4 * g4 + r, len - 1);
+          zw[t][r] = *reinterpret_cast<const uint32_t*>(ro.z + ((uint32_t)i * (uint32_t)p.z_stride + col));
+        }
+    }
+  };
+  if constexpr (!LATE) {
+    load_v();
+    load_z();
   }
   __builtin_amdgcn_sched_barrier(0);   // the loads stay where they stand
 
@@ -361,6 +371,10 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
     }
   }
   lds_barrier();
+  if constexpr (LATE) {
+    load_v();
+    __builtin_amdgcn_sched_barrier(0);
+  }
 
   const auto k_part = [&](int t, int s) { return load_bf16x8(&lds.k[kq_at(16 * t + c, 4 * s + g4)]); };
   const auto q_part = [&](int t, int s) { return load_bf16x8(&lds.q[kq_at(16 * t + c, 4 * s + g4)]); };
@@ -470,6 +484,10 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
         }
     }
     __builtin_amdgcn_sched_barrier(0);   // the parts of one step at a time in registers
+  }
+  if constexpr (LATE) {
+    load_z();
+    __builtin_amdgcn_sched_barrier(0);
   }
   // ---- R, and the state's part of the outputs ----
 #pragma unroll
