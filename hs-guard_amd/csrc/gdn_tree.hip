@@ -19,11 +19,11 @@
 // so U never leaves the registers; A, P and the inverses of A's diagonal blocks go through LDS as fp32.
 // G is summed and its differences taken in fp64: a steep decay early on a path must not cost the digits of the later ones.
 //
-// Bound by reading the state where trees are small (352 x 1 node, 16 value heads, fp32: 61 us, 6.1 TB/s; 68 without
-// nontemporal loads), by the issue of a CU's two or three workgroups where they are large: 128 x 64 nodes with commits 102 us
-// for 380 MB. A workgroup then lives 22 us, 6.4 of them until its loads are there, 2.7 in the coefficients, 2.7 in the
-// state's products, 1.8 in U, 2 in the commit; its products alone are 4.7. LDS reads ahead of the products and priorities of
-// the waves changed nothing; 8 waves of 16 columns spilled (125 -> 166 us).
+// Bound by reading the state where trees are small (352 x 1 node, 16 value heads, fp32: 59 us, 6.4 TB/s; 67 without
+// nontemporal loads), by the issue of a CU's two or three workgroups where they are large: 128 x 64 nodes with commits 93 us
+// for 380 MB. A workgroup then lives 20 us, 6 of them until its loads are there, 2 in the coefficients, 2.7 in the state's
+// products, 1.9 in U, 2.2 in the commit; its products alone are 4.7. LDS reads ahead of the products and priorities of the
+// waves changed nothing; 8 waves of 16 columns spilled (125 -> 166 us).
 //
 // A masked pair has a coefficient of 0, which would carry a NaN or an infinity of one branch to all others: where a result
 // is not finite, the workgroup computes its row again by walking each node's own ancestors (walk_row).
@@ -221,7 +221,7 @@ constexpr int occupancy(int nt, bool half) {
 }
 
 // NT: tiles of 16 nodes. One tile over an fp32 state does not move it: S0's registers are free as it is split, and four
-// workgroups on a CU instead of three (352 x 1 node 61 against 70 us; with commits two tiles were as fast, 112 and 112 us,
+// workgroups on a CU instead of three (352 x 1 node 59 against 67 us; with commits two tiles were as fast, 112 and 112 us,
 // and at 12 nodes faster, 154 and 157).
 template <int NT, bool HALF, bool GATED>
 __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(const TreeStepParams p) {
@@ -705,9 +705,9 @@ extern "C" int hsg_gdn_tree_step(const void* qkv, int64_t qkv_stride, int32_t q_
     if (state_dtype == HSG_STATE_F16) z ? launch(gdn_tree_kernel<NT, true, true>) : launch(gdn_tree_kernel<NT, true, false>);
     else z ? launch(gdn_tree_kernel<NT, false, true>) : launch(gdn_tree_kernel<NT, false, false>);
   };
-  // Tiles by the bound on a row's nodes: registers and LDS decide how many workgroups a CU holds. 352 x 1, fp16 state: 51 us with
-  // one tile, 54.5 with two; 200 x 24 with commits 88 with two, 106 with three; 96 x 33, fp16, 32 value heads 83 with three, 97
-  // with four.
+  // Tiles by the bound on a row's nodes: registers and LDS decide how many workgroups a CU holds. 352 x 1, fp16 state: 49 us
+  // with one tile, 51.5 with two; 200 x 24 with commits 84 with two, 92.5 with three; 96 x 33, fp16, 32 value heads 72 with
+  // three, 86 with four.
   if (max_nodes <= 16 && (state_dtype == HSG_STATE_F16 || !commits)) by_type(std::integral_constant<int, 1>{});
   else if (max_nodes <= 32) by_type(std::integral_constant<int, 2>{});
   else if (max_nodes <= 48) by_type(std::integral_constant<int, 3>{});
