@@ -220,7 +220,8 @@ def calls():
 
 
 def tensor_checks():
-    """The native checks of the operators' tensors (hs_guard._hsgtensor): ``operands`` and ``row_stride``."""
+    """The native checks of the operators' tensors and their outputs (hs_guard._hsgtensor): ``operands``, ``row_stride``,
+    ``empties``, ``empty_rows``."""
     global _tensor_checks
     if _tensor_checks is None:
         import torch  # noqa: F401  (its libraries, which the module is linked to)
