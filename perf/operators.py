@@ -176,19 +176,11 @@ def prepare(case, seed):
 # ---------------------------------------------------------------------------------------------------------------
 # One pass
 # ---------------------------------------------------------------------------------------------------------------
-_imported = None
-
-
 def _kernels():
-    """The framework's wrappers, imported once, as a program does."""
-    global _imported
-    if _imported is not None:
-        return _imported
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hs-guard_amd")
     if path not in sys.path:
         sys.path.insert(0, path)
     from hs_guard.engine import kernels
-    _imported = kernels
     return kernels
 
 
