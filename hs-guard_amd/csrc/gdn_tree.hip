@@ -130,6 +130,23 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&out)[PARTS]
   }
 }
 
+// Rows of T = (I + A_bb)^-1 from x = -A_bb: row i of T is e_i plus the sum of x_ik (row k of T) over k < i. Lane (g, c) holds
+// x's row c and columns 4 g .. 4 g + 3 of T's row c; step K gives row K, settled by then, to the rows below it (x_cK is 0 for
+// c <= K), as a broadcast within 16 lanes that the product takes as a modifier. Each row is a sum of what the solve itself
+// is a sum of, so nothing grows that has to cancel: chains of 16 to 64 nodes whose keys resemble one another leave their
+// state as exact as the step-by-step recurrence does (2e-7 to 7e-7). The product (I + x)(I + x^2)(I + x^4)(I + x^8) does not:
+// the powers' entries there are binomials up to 3,400 that cancel to order 1, and the state was off by 1e-5 to 3.5e-4. (15
+// dependent steps are also shorter than its three rounds of fp32 products: 128 x 64 nodes 93.5 -> 91.9 us, 96 x 33 71.3 -> 68.4.)
+template <int K = 0>
+__device__ __forceinline__ void substitute(const f32x4 (&x)[4], f32x4& t, int rows) {
+  if constexpr (K < 15) {
+    if (K % 4 == 0 && K + 1 >= rows) return;   // rows past the tree's end are 0 in x
+#pragma unroll
+    for (int r = 0; r < 4; ++r) t[r] = __builtin_fmaf(x[K / 4][K % 4], dpp_<0x150 + K>(t[r]), t[r]);   // row_newbcast:K
+    substitute<K + 1>(x, t, rows);
+  }
+}
+
 __device__ __forceinline__ float state_at(const void* state, bool half, int64_t at) {
   return half ? h2f(static_cast<const uint16_t*>(state)[at]) : static_cast<const float*>(state)[at];
 }
@@ -422,34 +439,15 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
   }
   lds_barrier();
 
-  // ---- the inverses of the diagonal blocks. X = -A_bb has X^16 = 0: (I - X)^-1 = (I + X)(I + X^2)(I + X^4)(I + X^8). x holds
-  // X in the accumulators' layout (x[r] = X[4 g4 + r][c], a B operand as it lies), y its transpose (y[r] = X[c][4 g4 + r], an A
-  // operand); each product of one with the other gives the next power of either. Rows past the tree's end are 0 in X. ----
+  // ---- the inverses of the diagonal blocks, by forward substitution: every lane has 4 columns of its row c of T ----
   const auto inverse = [&](int blk) {
-    f32x4 x, y = *reinterpret_cast<const f32x4*>(&lds.A[16 * blk + c][16 * blk + 4 * g4]);
+    f32x4 t, x[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = lds.A[16 * blk + 4 * g4 + r][16 * blk + c];
-    f32x4 z = y;                                        // transposed: the A operand of the products with T
+    for (int m = 0; m < 4; ++m) x[m] = *reinterpret_cast<const f32x4*>(&lds.A[16 * blk + c][16 * blk + 4 * m]);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) z[r] += 4 * g4 + r == c ? 1.f : 0.f;
-    const int rows = len - 16 * blk;
-#pragma unroll
-    for (int far = 2; far < 16; far <<= 1) {
-      if (far >= rows) break;
-      f32x4 x2 = {0.f, 0.f, 0.f, 0.f}, y2 = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x2 = __builtin_amdgcn_mfma_f32_16x16x4f32(y[r], x[r], x2, 0, 0, 0);
-        y2 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], y[r], y2, 0, 0, 0);
-      }
-      x = x2;
-      y = y2;
-      f32x4 z2 = z;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) z2 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], z[r], z2, 0, 0, 0);
-      z = z2;
-    }
-    return z;
+    for (int r = 0; r < 4; ++r) t[r] = 4 * g4 + r == c ? 1.f : 0.f;
+    substitute(x, t, len - 16 * blk);
+    return t;
   };
   f32x4 t0 = {0.f, 0.f, 0.f, 0.f};
   if constexpr (NT == 1) t0 = inverse(0);
