@@ -593,7 +593,9 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
   if (MOVES && ro.done > 0) {
     const float ec = lds.eG[ro.done - 1];
     constexpr int NP = (NT + 1) / 2;     // pairs of tiles: a product takes 32 nodes, the lane's own 4 of either tile
-    constexpr int U_PARTS = HALF ? 2 : 3;   // to an fp16 state, which keeps 11 digits, 16 of u (96 x 33 nodes 82 -> 80 us)
+    // (an fp16 state takes u with all its digits too: the 16 of two parts, cut off, made every update smaller and moved values
+    // by up to 1.2e-4 of their row beyond fp16's own rounding, against 4e-6; 96 x 33 nodes 68.4 -> 70.4 us)
+    constexpr int U_PARTS = 3;
     bf16x8 up[NP][2][U_PARTS];
 #pragma unroll
     for (int t2 = 0; t2 < NP; ++t2) {

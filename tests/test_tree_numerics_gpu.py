@@ -47,8 +47,18 @@ def check(s, rows, HV, most, slots):
 
 @pytest.mark.parametrize("n", [3, 9, 16, 33, 48, 64])
 @pytest.mark.parametrize("noise", [0.0, 0.05, 0.1])
-def test_chains_of_like_keys(n, noise):
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_chains_of_like_keys(n, noise, dtype):
     """Text that repeats itself, committed whole: what the chain's products do must not cancel."""
-    s = like_keys(n, n, 2, noise)
+    s = like_keys(n, n, 2, noise, dtype)
     for most in sorted({n, 64}):
         check(s, [(0, list(range(-1, n - 1)), n)], 2, most, [1])
+
+
+@pytest.mark.parametrize("n", [1, 3, 12, 17, 40, 64])
+def test_an_fp16_state_takes_whole_updates(n):
+    """Chains of unlike keys over an fp16 state, committed whole and in part: rounded once, from fp32's digits."""
+    s = like_keys(2 + n, n, 2, 1.0, torch.float16)
+    for done in sorted({1, (n + 1) // 2, n}):
+        for most in sorted({n, 64}):
+            check(s, [(0, list(range(-1, n - 1)), done)], 2, most, [0])
