@@ -157,53 +157,85 @@ __device__ __forceinline__ float log_decay(float a, float a_log, float dt_bias) 
 }
 
 // The row by its definition, node by node over each one's own ancestors: nothing is multiplied by a masked 0, and decays
-// are sums over the nodes between rather than differences. Thread t < 128 takes column t.
+// are sums over the nodes between rather than differences. Of each node, four threads an ancestor make its two products, and
+// thread t < 128 takes column t. One session whose state holds a NaN comes here in every layer and call, and all others of the
+// call wait for it: a row of 64 nodes 15.0 ms where every thread made all products by itself, from memory, 0.5 now.
 template <int NT, bool HALF, bool GATED>
-__device__ __forceinline__ void walk_row(const TreeStepParams& p, const TreeRow& ro, TreeStepLds<NT>& lds) {
-  const int col = threadIdx.x & (KD - 1);
-  const bool mine = threadIdx.x < KD;
-  const auto dot = [](const uint16_t* x, const uint16_t* y) {
-    float s = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < KD; ++k) s = __builtin_fmaf(bf2f(x[k]), bf2f(y[k]), s);
-    return s;
-  };
+__device__ __forceinline__ void walk_row(const TreeStepParams& p, const TreeRow& ro, TreeStepLds<NT>& lds, int tid) {
+  const int col = tid & (KD - 1);
+  const bool mine = tid < KD;
   const auto between = [&](uint64_t nodes) {
     float s = 0.f;
+#pragma unroll 1
     for (; nodes; nodes &= nodes - 1) s += lds.g[__builtin_ctzll(nodes)];
-    return expf(s);
+    return s;
   };
-  __syncthreads();   // P, which U lies over, is read no more
+#pragma unroll 1
   for (int i = 0; i < ro.len; ++i) {
     const uint64_t path = lds.mask[i];
-    const uint16_t* ki = ro.k + i * p.qkv_stride;
-    const uint16_t* qi = ro.q + i * p.qkv_stride;
+    // the ancestors' products: thread 4 j + e has dims 32 e .. of node j's, and the decays of nodes 16 e .. between
+    __syncthreads();   // P, which U lies over, and the coefficients of the node before are read no more
+    {
+      const int j = tid >> 2, e = tid & 3;
+      const bool on = j <= i && (path >> j & 1u);
+      float kk = 0.f, qk = 0.f, g = 0.f;
+      if (on) {
+#pragma unroll 1
+        for (int pc = 4 * e; pc < 4 * e + 4; ++pc) {
+          float x[8], y[8], z[8];
+          load8_bf16(&lds.k[kq_at(j, pc)], x);
+          load8_bf16(&lds.k[kq_at(i, pc)], y);
+          load8_bf16(&lds.q[kq_at(i, pc)], z);
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            kk = __builtin_fmaf(x[d], y[d], kk);
+            qk = __builtin_fmaf(x[d], z[d], qk);
+          }
+        }
+        g = between(path & ~lds.mask[j] & (0xffffull << (16 * e)));
+      }
+      kk = add_xor2(add_xor1(kk));
+      qk = add_xor2(add_xor1(qk));
+      g = add_xor2(add_xor1(g));
+      if (on && e == 0) {
+        const float d = expf(g) * lds.kinv[j];
+        lds.part[j][2] = d * lds.kinv[i] * kk;
+        lds.part[j][3] = d * lds.qinv[i] * qk;
+      }
+    }
+    __syncthreads();
     float o = 0.f;
     if (mine) {
       float ks = 0.f, qs = 0.f;
-#pragma unroll 4
-      for (int k = 0; k < KD; ++k) {
-        const float s = state_at(p.state, HALF, ro.state_at + (int64_t)k * KD + col);
-        ks = __builtin_fmaf(bf2f(ki[k]), s, ks);
-        qs = __builtin_fmaf(bf2f(qi[k]), s, qs);
+#pragma unroll 1
+      for (int pc = 0; pc < KD / 8; ++pc) {
+        float x[8], y[8];
+        load8_bf16(&lds.k[kq_at(i, pc)], x);
+        load8_bf16(&lds.q[kq_at(i, pc)], y);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const float s = state_at(p.state, HALF, ro.state_at + (int64_t)(8 * pc + d) * KD + col);
+          ks = __builtin_fmaf(x[d], s, ks);
+          qs = __builtin_fmaf(y[d], s, qs);
+        }
       }
-      const float e = between(path);
+      const float e = expf(between(path));
       float read = e * lds.kinv[i] * ks;
       o = e * lds.qinv[i] * qs;
+#pragma unroll 1
       for (uint64_t up = path & ~(1ull << i); up; up &= up - 1) {
         const int j = __builtin_ctzll(up);
-        const uint16_t* kj = ro.k + j * p.qkv_stride;
-        const float d = between(path & ~lds.mask[j]) * lds.kinv[j];
-        read += d * lds.kinv[i] * dot(ki, kj) * lds.U[j][col];
-        o += d * lds.qinv[i] * dot(qi, kj) * lds.U[j][col];
+        const float u = lds.U[j][col];
+        read = __builtin_fmaf(lds.part[j][2], u, read);
+        o = __builtin_fmaf(lds.part[j][3], u, o);
       }
       const float u = lds.beta[i] * (bf2f(ro.v[i * p.qkv_stride + col]) - read);
       lds.U[i][col] = u;
-      o += lds.qinv[i] * lds.kinv[i] * dot(qi, ki) * u;
+      o = __builtin_fmaf(lds.part[i][3], u, o);
     }
     if constexpr (GATED) {
       const float ss = wave_sum(o * o);
-      if (mine && (threadIdx.x & 63) == 0) lds.part[i][threadIdx.x >> 6] = ss;
+      if (mine && (tid & 63) == 0) lds.part[i][tid >> 6] = ss;
       __syncthreads();
       if (mine) {
         const float r = rsqrtf((lds.part[i][0] + lds.part[i][1]) * (1.0f / KD) + p.eps);
@@ -215,18 +247,30 @@ __device__ __forceinline__ void walk_row(const TreeStepParams& p, const TreeRow&
   if (ro.done > 0) {
     const int c = ro.done - 1;
     __syncthreads();   // the sums of squares are read no more
-    for (int j = threadIdx.x; j < ro.done; j += 64 * NW)
-      lds.part[j][0] = between(lds.mask[c] & ~lds.mask[j]) * lds.kinv[j];
+    for (int j = tid; j < ro.done; j += 64 * NW)
+      lds.part[j][0] = expf(between(lds.mask[c] & ~lds.mask[j])) * lds.kinv[j];
     __syncthreads();
     if (mine) {
-      const float e = between(lds.mask[c]);
-      for (int k = 0; k < KD; ++k) {
-        const int64_t at = ro.state_at + (int64_t)k * KD + col;
-        float s = e * state_at(p.state, HALF, at);
-        for (int j = 0; j < ro.done; ++j)
-          s = __builtin_fmaf(lds.part[j][0] * bf2f(ro.k[j * p.qkv_stride + k]), lds.U[j][col], s);
-        if constexpr (HALF) static_cast<uint16_t*>(p.state)[at] = f2h(s);
-        else static_cast<float*>(p.state)[at] = s;
+      const float e = expf(between(lds.mask[c]));
+#pragma unroll 1
+      for (int pc = 0; pc < KD / 8; ++pc) {
+        const int64_t at = ro.state_at + (int64_t)(8 * pc) * KD + col;
+        float s[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) s[d] = e * state_at(p.state, HALF, at + d * KD);
+#pragma unroll 1
+        for (int j = 0; j < ro.done; ++j) {
+          const float w = lds.part[j][0], u = lds.U[j][col];
+          float x[8];
+          load8_bf16(&lds.k[kq_at(j, pc)], x);
+#pragma unroll
+          for (int d = 0; d < 8; ++d) s[d] = __builtin_fmaf(w * x[d], u, s[d]);
+        }
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          if constexpr (HALF) static_cast<uint16_t*>(p.state)[at + d * KD] = f2h(s[d]);
+          else static_cast<float*>(p.state)[at + d * KD] = s[d];
+        }
       }
     }
   }
@@ -557,7 +601,10 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
   if (lane == 0) lds.odd[wave] = bad != 0;
   __syncthreads();
   if (lds.odd[0] | lds.odd[1] | lds.odd[2] | lds.odd[3]) {
-    walk_row<NT, HALF, GATED>(p, ro, lds);
+    // (the arguments are read again: kept until here, with all that this takes, they cost a register spill)
+    const auto* args = (const __attribute__((address_space(4))) TreeStepParams*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    walk_row<NT, HALF, GATED>(*(const TreeStepParams*)args, ro, lds, 64 * wave + lane_per_site(lane));
     return;
   }
 
