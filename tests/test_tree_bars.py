@@ -102,6 +102,17 @@ def test_mistakes_deep_in_a_tree_are_seen(mistake):
             assert norm > 4 * STATE_NORM or "output" in mistake
 
 
+@pytest.mark.parametrize("n", [20, 64])
+def test_steep_decays_pass(n):
+    s = like_keys(n, n, 1, 1.0)
+    s["A_log"][:] = 2.7
+    for at, a in ((n // 3, 8.0), (n // 2, 47.0), (n - 2, 8.0)):
+        s["a"][at] = a
+    for done in (n, n // 2):
+        norm, out, value = errors(s, list(range(-1, n - 1)), done)
+        assert norm < STATE_NORM and out < VALUE and value < VALUE
+
+
 @pytest.mark.parametrize("n", [1, 3, 12, 40])
 def test_an_fp16_state_tells_an_update_of_16_digits(n):
     """What fp32 leaves moves few values over a border of fp16, and these by little."""
