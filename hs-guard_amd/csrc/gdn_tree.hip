@@ -16,14 +16,16 @@
 // k and q are exact in bf16 and their lengths divide the products afterwards; a state value is split into three bf16 parts
 // (two from fp16) that hold all its digits, so S0^T k is as exact as fp32 products. k.k and q.k are bf16 products, exact up
 // to fp32 sums. U and the accumulators share the MFMA layout (a lane's 4 registers are 4 consecutive nodes of one column),
-// so U never leaves the registers; A, P and the inverses of A's diagonal blocks go through LDS as fp32.
+// so U never leaves the registers; A, P and the inverses of A's diagonal blocks go through LDS as fp32. A committed state is
+// as exact as the step-by-step fp32 recurrence leaves it, also where a path's keys resemble one another (substitute below).
 // G is summed and its differences taken in fp64: a steep decay early on a path must not cost the digits of the later ones.
 //
 // Bound by reading the state where trees are small (352 x 1 node, 16 value heads, fp32: 59 us, 6.4 TB/s; 67 without
-// nontemporal loads), by the issue of a CU's two or three workgroups where they are large: 128 x 64 nodes with commits 93 us
-// for 380 MB. A workgroup then lives 20 us, 6 of them until its loads are there, 2 in the coefficients, 2.7 in the state's
-// products, 1.9 in U, 2.2 in the commit; its products alone are 4.7. LDS reads ahead of the products and priorities of the
-// waves changed nothing; 8 waves of 16 columns spilled (125 -> 166 us).
+// nontemporal loads), by the issue of a CU's two workgroups where they are large: 128 x 64 nodes with commits 91 us for 380
+// MB. A workgroup then lives 20 us, 6 of them until its loads are there, 2 in the coefficients, 2.7 in the state's products,
+// 1.9 in U, 2.2 in the commit; its products alone are 4.7. LDS reads ahead of the products and priorities of the waves
+// changed nothing; 8 waves of 16 columns spilled (a third slower). Over an fp16 state a wave's 32 columns are half a line,
+// which nontemporal accesses move twice: 96 x 33 nodes, 32 value heads, 69 us for 331 MB moved where 263 are needed.
 //
 // A masked pair has a coefficient of 0, which would carry a NaN or an infinity of one branch to all others: where a result
 // is not finite, the workgroup computes its row again by walking each node's own ancestors (walk_row).
@@ -282,8 +284,8 @@ constexpr int occupancy(int nt, bool half) {
 }
 
 // NT: tiles of 16 nodes. One tile over an fp32 state does not move it: S0's registers are free as it is split, and four
-// workgroups on a CU instead of three (352 x 1 node 59 against 67 us; with commits two tiles were as fast, 112 and 112 us,
-// and at 12 nodes faster, 154 and 157).
+// workgroups on a CU instead of three (352 x 1 node 59 against 67 us; with commits two tiles were as fast, and at 12 nodes
+// 2 % faster).
 template <int NT, bool HALF, bool GATED>
 __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(const TreeStepParams p) {
   constexpr bool MOVES = HALF || NT > 1;
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
   };
   // ---- v and z ----
   // A wave has at most 63 loads on their way: with more than a tile it would stand here until the first are back, so that
-  // there v is loaded after the first barrier and z after the state's products (96 x 33 76 -> 73 us, 128 x 64 106 -> 103.5).
+  // there v is loaded after the first barrier and z after the state's products (96 x 33 nodes 4 % faster, 128 x 64 2 %).
   constexpr bool LATE = NT > 1;
   uint32_t vw[NT][4], zw[GATED ? NT : 1][4], nw = 0;
   const auto load_v = [&]() __attribute__((always_inline)) {
@@ -641,7 +643,7 @@ __global__ __launch_bounds__(64 * NW, occupancy(NT, HALF)) void gdn_tree_kernel(
     const float ec = lds.eG[ro.done - 1];
     constexpr int NP = (NT + 1) / 2;     // pairs of tiles: a product takes 32 nodes, the lane's own 4 of either tile
     // (an fp16 state takes u with all its digits too: the 16 of two parts, cut off, made every update smaller and moved values
-    // by up to 1.2e-4 of their row beyond fp16's own rounding, against 4e-6; 96 x 33 nodes 68.4 -> 70.4 us)
+    // by up to 1.2e-4 of their row beyond fp16's own rounding, where 7.6e-6 is the bar now; 96 x 33 nodes 68.4 -> 70.4 us)
     constexpr int U_PARTS = 3;
     bf16x8 up[NP][2][U_PARTS];
 #pragma unroll
@@ -752,9 +754,9 @@ extern "C" int hsg_gdn_tree_step(const void* qkv, int64_t qkv_stride, int32_t q_
     if (state_dtype == HSG_STATE_F16) z ? launch(gdn_tree_kernel<NT, true, true>) : launch(gdn_tree_kernel<NT, true, false>);
     else z ? launch(gdn_tree_kernel<NT, false, true>) : launch(gdn_tree_kernel<NT, false, false>);
   };
-  // Tiles by the bound on a row's nodes: registers and LDS decide how many workgroups a CU holds. 352 x 1, fp16 state: 49 us
-  // with one tile, 51.5 with two; 200 x 24 with commits 84 with two, 92.5 with three; 96 x 33, fp16, 32 value heads 72 with
-  // three, 86 with four.
+  // Tiles by the bound on a row's nodes: registers and LDS decide how many workgroups a CU holds. 352 x 1, fp16 state: 46 us
+  // with one tile, 49 with two, 55 with three; 200 x 24 with commits 82.6 with two, 85.2 with three; 96 x 33, fp16, 32 value
+  // heads, 68.6 with three, 79.7 with four (fp32, 16 heads 49.7 and 51.8).
   if (max_nodes <= 16 && (state_dtype == HSG_STATE_F16 || !commits)) by_type(std::integral_constant<int, 1>{});
   else if (max_nodes <= 32) by_type(std::integral_constant<int, 2>{});
   else if (max_nodes <= 48) by_type(std::integral_constant<int, 3>{});
